@@ -200,6 +200,42 @@ int moe_rmsnorm_bwd(const void* dx, const void* dx2, const void* h,
                     void* dh, void* dgamma, void* workspace,
                     size_t workspace_bytes, void* stream);
 
+/* The residual stream between two blocks, per row in fp32:
+ *   v = y * ry * post (ry = rsqrt(mean(y^2) + eps)), or y where post is NULL;
+ *   h = residual_scale * residual + branch_scale * g * v;
+ *   r = rsqrt(mean(h^2) + eps);  hidden = h, x = h * r * gamma, rounded once each.
+ * gate_kind: 0 no gate (g = 1, gate NULL), 1 one g per row (gate[T]), 2 one per
+ * column (gate[H]), 3 one per element (gate[T,H]).  All operands bf16, or all
+ * f32 with is_f32; rstd_y[T] (written with post only) and rstd[T] are f32.
+ * H a multiple of 8, at most 8192.  For eps = 1e-6, equal scales of 1, no post
+ * and no gate, hidden and x are the sum and the norm of
+ * TF/models/qwen3_moe/modeling_qwen3_moe.py:340-345 with one rounding. */
+int moe_residual_norm_fwd(const void* y, const void* residual, const void* post,
+                          const void* gate, int gate_kind, const void* gamma,
+                          int is_f32, int64_t T, int64_t H, float branch_scale,
+                          float residual_scale, float eps, void* hidden,
+                          void* x, float* rstd_y, float* rstd, void* stream);
+
+/* Backward of moe_residual_norm_fwd, from the same operands and its rstd_y
+ * and rstd: with e = d_x * gamma,
+ *   dh = d_hidden + r e - (r^3 / H) h sum_j e_j h_j  (d_hidden or d_x NULL: zero),
+ *   d_residual = residual_scale dh;  dz = branch_scale g dh;
+ *   d_y = dz, or with post and f = dz post, ry f - (ry^3 / H) y sum_j f_j y_j;
+ *   d_gate = branch_scale dh v, summed over what a gate value covers;
+ *   d_post = sum_t dz y ry;  d_gamma = sum_t d_x h r  (fixed-order sums).
+ * Without post and gate d_y or d_residual may be NULL (not written).  With
+ * T = 0 the vectors' gradients are zeros. */
+size_t moe_residual_norm_bwd_workspace_bytes(int64_t T, int64_t H);
+int moe_residual_norm_bwd(const void* d_hidden, const void* d_x, const void* y,
+                          const void* residual, const void* post,
+                          const void* gate, int gate_kind, const void* gamma,
+                          const float* rstd_y, const float* rstd, int is_f32,
+                          int64_t T, int64_t H, float branch_scale,
+                          float residual_scale, void* d_y, void* d_residual,
+                          void* d_post, void* d_gate, void* d_gamma,
+                          void* workspace, size_t workspace_bytes,
+                          void* stream);
+
 /* moe_router_fwd plus the Switch aux loss of moe_aux_loss_fwd (same aux and
  * stats outputs, token_weight as there) from the router's own softmax and
  * top-k, where the reference recomputes both from the logits

@@ -27,6 +27,7 @@ from .moe import (
     mi355x_experts_forward,
     register_experts_implementation,
 )
+from .residual_norm import residual_norm
 from .token_dispatch import DispatchState, TokenDispatcher, variable_all_to_all
 
 __all__ = [
@@ -50,6 +51,7 @@ __all__ = [
     "local_expert_range",
     "mi355x_experts_forward",
     "register_experts_implementation",
+    "residual_norm",
     "sequence_parallel_load_balancing_loss",
     "variable_all_to_all",
     "verify_expert_modules",

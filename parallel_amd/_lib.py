@@ -30,6 +30,7 @@ _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/moe_mi355x.h one to one.
 SIGNATURES: dict[str, tuple] = {
@@ -75,6 +76,10 @@ SIGNATURES: dict[str, tuple] = {
     "moe_rmsnorm_fwd": (_I, [_P, _P, _I64, _I64, ctypes.c_float, _P, _P, _P]),
     "moe_rmsnorm_bwd_workspace_bytes": (_SZ, [_I64, _I64]),
     "moe_rmsnorm_bwd": (_I, [_P, _P, _P, _P, _P, _I64, _I64, _P, _P, _P, _SZ, _P]),
+    "moe_residual_norm_fwd": (_I, [_P, _P, _P, _P, _I, _P, _I, _I64, _I64, _F, _F, _F, _P, _P, _P, _P, _P]),
+    "moe_residual_norm_bwd_workspace_bytes": (_SZ, [_I64, _I64]),
+    "moe_residual_norm_bwd": (_I, [_P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I64, _I64, _F, _F, _P, _P, _P, _P, _P,
+                                   _P, _SZ, _P]),
     "moe_router_aux_fwd_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
     "moe_router_aux_fwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _SZ, _P]),
 }

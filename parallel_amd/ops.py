@@ -17,6 +17,7 @@ Ops (namespace ``parallel_amd``):
   rmsnorm_fwd / rmsnorm_bwd        post_attention_layernorm of the block input (+ backward)
   router_aux_fwd                   router_fwd plus the aux loss from the same top-k
   moe_block_fwd                    router, aux loss and experts as one op (moe_block)
+  residual_norm_fwd / _bwd         a block's output normed, gated, added to the residual, and the sum normed
 
 experts_bwd_kernels issues the expert backward's launches with a caller-chosen
 weight-gradient target (fsdp_bucket uses it to write into an FSDP bucket).
@@ -25,6 +26,7 @@ weight-gradient target (fsdp_bucket uses it to write into an FSDP bucket).
 from __future__ import annotations
 
 import inspect
+from contextlib import nullcontext
 
 import torch
 from torch import Tensor
@@ -141,8 +143,29 @@ def _stream(t: Tensor) -> int:
     return _lib.stream_of(t)
 
 
+def _require_one_device(*tensors: Tensor | None) -> None:
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) > 1:
+        raise ValueError(f"tensors are on different devices: {sorted(map(str, devices))}")
+
+
+def _device(t: Tensor):
+    """Makes the tensor's GPU the current one for launches on its stream (nothing to do where it is already)."""
+    return nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
 def _ws(nbytes: int, device) -> Tensor:
     return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def _rows16(t: Tensor) -> Tensor:
+    """Contiguous rows at the 16-byte aligned address that the kernels load from."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _rows16_opt(t: Tensor | None) -> Tensor | None:
+    return None if t is None else _rows16(t)
 
 
 def _ids64(t: Tensor) -> Tensor:
@@ -612,6 +635,137 @@ def _router_aux_backward(ctx, d_logits, d_scores, _d_idx, d_aux, _d_stats):
 
 router_aux_fwd.register_autograd(_router_aux_backward, setup_context=_router_aux_setup)
 run_router_aux_fwd = _eager_route("router_aux_fwd", router_aux_fwd, _router_aux_setup, _router_aux_backward)
+
+
+# --------------------------------------------- the residual stream around a block
+
+_RESIDUAL_NORM_DTYPES = (BF16, torch.float32)
+_GATES = ("none", "token", "channel", "full")
+
+
+def _gate_kind(y: Tensor, gate: Tensor | None) -> int:
+    if gate is None:
+        return 0
+    H = y.shape[-1]
+    if gate.shape == y.shape[:-1] + (1,):
+        return 1
+    if gate.shape == (H,):
+        return 2
+    if gate.shape == y.shape:
+        return 3
+    raise ValueError(f"gate must be {tuple(y.shape[:-1]) + (1,)} (per token), ({H},) (per channel) or "
+                     f"{tuple(y.shape)}, got {tuple(gate.shape)}")
+
+
+def _check_residual_norm(y, residual, weight, post_weight, gate) -> int:
+    if y.dim() < 1 or residual.shape != y.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} does not match the block's output {tuple(y.shape)}")
+    if y.dtype not in _RESIDUAL_NORM_DTYPES:
+        raise ValueError(f"residual_norm takes bfloat16 or float32, got {y.dtype}")
+    for name, t in (("residual", residual), ("weight", weight), ("post_weight", post_weight), ("gate", gate)):
+        if t is not None and t.dtype != y.dtype:
+            raise ValueError(f"{name} must be {y.dtype} as the block's output is, got {t.dtype}")
+    H = y.shape[-1]
+    for name, t in (("weight", weight), ("post_weight", post_weight)):
+        if t is not None and t.shape != (H,):
+            raise ValueError(f"{name} must be ({H},), got {tuple(t.shape)}")
+    kind = _gate_kind(y, gate)
+    _require_gpu(y, residual, weight, post_weight, gate)
+    _require_one_device(y, residual, weight, post_weight, gate)
+    return kind
+
+
+@_op("residual_norm_fwd")
+def residual_norm_fwd(y: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None,
+                      branch_scale: float, residual_scale: float, eps: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(hidden, x, rstd_y [T] f32 (empty without post_weight), rstd [T] f32): see residual_norm.residual_norm."""
+    kind = _check_residual_norm(y, residual, weight, post_weight, gate)
+    H = y.shape[-1]
+    T = y.numel() // H if H else 0
+    f32 = dict(dtype=torch.float32, device=y.device)
+    hidden = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    x = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    rstd_y = torch.empty(0 if post_weight is None else T, **f32)
+    rstd = torch.empty(T, **f32)
+    y, residual, weight, post_weight, gate = map(_rows16_opt, (y, residual, weight, post_weight, gate))
+    with _device(y):
+        call("moe_residual_norm_fwd", ptr(y), ptr(residual), ptr(post_weight), ptr(gate), kind, ptr(weight),
+             int(y.dtype == torch.float32), T, H, branch_scale, residual_scale, eps, ptr(hidden), ptr(x), ptr(rstd_y),
+             ptr(rstd), _stream(y), tag="residual_norm_fwd")
+    return hidden, x, rstd_y, rstd
+
+
+@residual_norm_fwd.register_fake
+def _(y, residual, weight, post_weight, gate, branch_scale, residual_scale, eps):
+    T = y.numel() // y.shape[-1]
+    return (y.new_empty(y.shape), y.new_empty(y.shape),
+            y.new_empty(0 if post_weight is None else T, dtype=torch.float32), y.new_empty(T, dtype=torch.float32))
+
+
+@_op("residual_norm_bwd")
+def residual_norm_bwd(d_hidden: Tensor | None, d_x: Tensor | None, y: Tensor, residual: Tensor, weight: Tensor,
+                      post_weight: Tensor | None, gate: Tensor | None, rstd_y: Tensor, rstd: Tensor,
+                      branch_scale: float, residual_scale: float) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(d_y, d_residual, d_weight, d_post_weight, d_gate) of residual_norm_fwd; empty where there is no such
+    gradient, and d_y also where it equals d_residual (no post_weight, no gate, equal scales)."""
+    kind = _gate_kind(y, gate)
+    H = y.shape[-1]
+    T = y.numel() // H if H else 0
+    dev, dt = y.device, y.dtype
+    one = _one_input_gradient(post_weight, gate, branch_scale, residual_scale)
+    d_residual = torch.empty(y.shape, dtype=dt, device=dev)
+    d_y = torch.empty(0 if one else y.shape, dtype=dt, device=dev)
+    d_weight = torch.empty(H, dtype=dt, device=dev)
+    d_post = torch.empty(0 if post_weight is None else H, dtype=dt, device=dev)
+    d_gate = torch.empty(0 if gate is None else gate.shape, dtype=dt, device=dev)
+    d_hidden, d_x = (None if d is None else _rows16(d.to(dt)) for d in (d_hidden, d_x))
+    y, residual, weight, post_weight, gate = map(_rows16_opt, (y, residual, weight, post_weight, gate))
+    with _device(y):
+        ws = _ws(_lib.load().moe_residual_norm_bwd_workspace_bytes(T, H), dev)
+        call("moe_residual_norm_bwd", ptr(d_hidden), ptr(d_x), ptr(y), ptr(residual), ptr(post_weight), ptr(gate),
+             kind, ptr(weight), ptr(rstd_y), ptr(rstd), int(dt == torch.float32), T, H, branch_scale, residual_scale,
+             None if one else ptr(d_y), ptr(d_residual), None if post_weight is None else ptr(d_post),
+             None if gate is None else ptr(d_gate), ptr(d_weight), ptr(ws), ws.numel(), _stream(y),
+             tag="residual_norm_bwd")
+    return d_y, d_residual, d_weight, d_post, d_gate
+
+
+def _one_input_gradient(post_weight, gate, branch_scale: float, residual_scale: float) -> bool:
+    return post_weight is None and gate is None and branch_scale == residual_scale
+
+
+@residual_norm_bwd.register_fake
+def _(d_hidden, d_x, y, residual, weight, post_weight, gate, rstd_y, rstd, branch_scale, residual_scale):
+    one = _one_input_gradient(post_weight, gate, branch_scale, residual_scale)
+    return (y.new_empty(0 if one else y.shape), y.new_empty(y.shape), weight.new_empty(weight.shape),
+            weight.new_empty(0 if post_weight is None else weight.shape),
+            y.new_empty(0 if gate is None else gate.shape))
+
+
+def _residual_norm_setup(ctx, inputs, output):
+    ctx.set_materialize_grads(False)
+    y, residual, weight, post_weight, gate, branch_scale, residual_scale, _eps = inputs
+    _, _, rstd_y, rstd = output
+    ctx.save_for_backward(y, residual, weight, post_weight, gate, rstd_y, rstd)
+    ctx.scales = (branch_scale, residual_scale)
+    ctx.mark_non_differentiable(rstd_y, rstd)
+
+
+def _residual_norm_backward(ctx, d_hidden, d_x, _d_rstd_y, _d_rstd):
+    if d_hidden is None and d_x is None:
+        return (None,) * 8
+    y, residual, weight, post_weight, gate, rstd_y, rstd = ctx.saved_tensors
+    d_y, d_res, d_w, d_post, d_gate = _direct("residual_norm_bwd", d_hidden, d_x, y, residual, weight, post_weight,
+                                              gate, rstd_y, rstd, *ctx.scales)
+    if _one_input_gradient(post_weight, gate, *ctx.scales):
+        d_y = d_res
+    return (d_y, d_res, d_w, None if post_weight is None else d_post, None if gate is None else d_gate,
+            None, None, None)
+
+
+residual_norm_fwd.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
+run_residual_norm_fwd = _eager_route("residual_norm_fwd", residual_norm_fwd, _residual_norm_setup,
+                                     _residual_norm_backward)
 
 
 # ------------------------------------------------------------------ permute
@@ -1285,12 +1439,6 @@ run_combine_rows_fwd = _eager_route("combine_rows_fwd", combine_rows_fwd, _combi
 # order's rows with the others' dropped or zero-filled (dispatch_fwd and
 # combine_rows_fwd around variable_all_to_all) give the same values and remain
 # for calls that the ops' route takes.
-
-
-def _rows16(t: Tensor) -> Tensor:
-    """Contiguous rows at the 16-byte aligned address that the kernels load from."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 class _ScatterBlock(torch.autograd.Function):
