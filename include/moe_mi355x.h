@@ -435,6 +435,53 @@ int moe_grouped_gemm_wgrad_bucket(const void* dc, const void* a,
                                   int64_t bucket_rows, int64_t bucket_stride,
                                   int dw_is_f32, int accumulate, void* stream);
 
+/* ---------------------------------------------- 4-bit microscaled operands (mx4) */
+
+/* A row of K values (K a multiple of 32) is K/2 bytes of codes (the value of
+ * even index in the low four bits of a byte: a sign bit and the index of 0,
+ * 0.5, 1, 1.5, 2, 3, 4, 6) and 8 * ceil(K/256) bytes of scales, of which byte
+ * j < K/32 is the exponent s of the values 32 j .. 32 j + 31: a value is its
+ * code times 2^(s - 127), or NaN where s is 255.  (The OCP microscaling
+ * format's E2M1 with E8M0 scales; the rest of a scale row is padding.)  Codes
+ * are 16-byte aligned, scales 8-byte aligned; rows lie end to end.  The
+ * reference has no such format.
+ *
+ * Quantisation of a block: s = max(floor(log2(largest size)) - 2 + 127, 0),
+ * every value divided by 2^(s - 127), rounded to the nearest code (ties to the
+ * even index) and clamped to 6; a block with an infinity or NaN gets s = 255
+ * and zero codes.  x is bf16, or f32 with is_f32; padding is written as 0. */
+int moe_mx4_quantize(const void* x, int is_f32, int64_t rows, int64_t K,
+                     void* codes, void* scales, void* stream);
+/* The values of codes and scales, bf16 (exact) or f32 with is_f32. */
+int moe_mx4_dequantize(const void* codes, const void* scales, int64_t rows,
+                       int64_t K, int is_f32, void* out, void* stream);
+
+/* Grouped products of mx4 operands, fp32 accumulation (v_mfma_scale_f32_*):
+ * c[r, n] = sum_k A[src(r), k] W[g][n, k] (bf16) for the rows r of group g
+ * (offs as in the grouped GEMMs above; rows at or beyond offs[G-1] are not
+ * touched), W [G, N, K].  src(r) = r, or row_index[r] / row_divisor when
+ * row_index is not NULL (the sort's perm and k: a token's row is then read for
+ * each of its slots); a source row outside [0, a_rows) counts as zeros.
+ * N a multiple of 8; A and each group's W below 2 GiB. */
+int moe_mx4_grouped_gemm(const void* a_codes, const void* a_scales,
+                         int64_t a_rows, const int32_t* row_index,
+                         int64_t row_divisor, const void* w_codes,
+                         const void* w_scales, const int32_t* offs, int64_t G,
+                         int64_t M, int64_t N, int64_t K, void* c,
+                         void* stream);
+
+/* act[r, i] = silu(gate) * up from the same product with W [G, 2I, K] (the
+ * first I rows are the gate), formed in fp32 and rounded once: to bf16 act, or
+ * where act_codes is not NULL to mx4 rows (I a multiple of 32; the padding of
+ * act_scales is not written). */
+int moe_mx4_grouped_swiglu(const void* a_codes, const void* a_scales,
+                           int64_t a_rows, const int32_t* row_index,
+                           int64_t row_divisor, const void* w_codes,
+                           const void* w_scales, const int32_t* offs,
+                           int64_t G, int64_t M, int64_t I, int64_t K,
+                           void* act, void* act_codes, void* act_scales,
+                           void* stream);
+
 /* ------------------------------------------------------ the fp32 expert path */
 
 /* The reference's grouped experts accept fp32 modules and then compute in

@@ -17,6 +17,8 @@ Ops (namespace ``parallel_amd``):
   rmsnorm_fwd / rmsnorm_bwd        post_attention_layernorm of the block input (+ backward)
   router_aux_fwd                   router_fwd plus the aux loss from the same top-k
   moe_block_fwd                    router, aux loss and experts as one op (moe_block)
+  mx4_quantize / mx4_dequantize    blocks of 32 values as 4-bit codes with a shared power-of-two scale
+  mx4_grouped_mm / mx4_grouped_swiglu / mx4_experts   products of such operands (inference; no gradients)
   residual_norm_fwd / _bwd         a block's output normed, gated, added to the residual, and the sum normed
 
 experts_bwd_kernels issues the expert backward's launches with a caller-chosen
@@ -766,6 +768,198 @@ def _residual_norm_backward(ctx, d_hidden, d_x, _d_rstd_y, _d_rstd):
 residual_norm_fwd.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
 run_residual_norm_fwd = _eager_route("residual_norm_fwd", residual_norm_fwd, _residual_norm_setup,
                                      _residual_norm_backward)
+
+
+# ------------------------------------------- 4-bit microscaled operands (mx4)
+#
+# A tensor [..., K] is codes uint8 [..., K/2] and scales uint8 [..., 8 ceil(K/256)]
+# (include/moe_mi355x.h states the format).  These ops have no gradients.
+
+
+def mx4_pitch(K: int) -> int:
+    """Bytes of a row's scales: one per 32 values, padded to 8 per 256."""
+    return 8 * -(-K // 256)
+
+
+def _check_mx4(name: str, codes: Tensor, scales: Tensor) -> int:
+    """K of an mx4 operand."""
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"{name}: codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
+    K = 2 * codes.shape[-1]
+    if K == 0 or K % 32:
+        raise ValueError(f"{name}: rows of {K} values are not whole blocks of 32")
+    if scales.shape != codes.shape[:-1] + (mx4_pitch(K),):
+        raise ValueError(f"{name}: scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}: rows of {K} "
+                         f"values have {mx4_pitch(K)} scale bytes")
+    return K
+
+
+def _refuse_gradients(what: str, *tensors: Tensor) -> None:
+    if _wants_grad(tensors):
+        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+@_op("mx4_quantize")
+def mx4_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    """(codes [..., K/2], scales [..., pitch]) of x [..., K], bfloat16 or float32."""
+    if x.dtype not in (BF16, torch.float32):
+        raise ValueError(f"mx4_quantize takes bfloat16 or float32, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise ValueError(f"mx4_quantize: rows of {tuple(x.shape)} are not whole blocks of 32 values")
+    _require_gpu(x)
+    K = x.shape[-1]
+    x = _rows16(x)
+    codes = torch.empty(x.shape[:-1] + (K // 2,), dtype=torch.uint8, device=x.device)
+    scales = torch.empty(x.shape[:-1] + (mx4_pitch(K),), dtype=torch.uint8, device=x.device)
+    with _device(x):
+        call("moe_mx4_quantize", ptr(x), int(x.dtype == torch.float32), x.numel() // K, K, ptr(codes), ptr(scales),
+             _stream(x), tag="mx4_quantize")
+    return codes, scales
+
+
+@mx4_quantize.register_fake
+def _(x):
+    K = x.shape[-1]
+    return (x.new_empty(x.shape[:-1] + (K // 2,), dtype=torch.uint8),
+            x.new_empty(x.shape[:-1] + (mx4_pitch(K),), dtype=torch.uint8))
+
+
+@_op("mx4_dequantize")
+def mx4_dequantize(codes: Tensor, scales: Tensor, float32: bool) -> Tensor:
+    """The values [..., K] of an mx4 tensor, bfloat16 (exact) or float32."""
+    K = _check_mx4("mx4_dequantize", codes, scales)
+    _require_gpu(codes, scales)
+    _require_one_device(codes, scales)
+    codes, scales = _rows16(codes), _rows16(scales)
+    out = torch.empty(codes.shape[:-1] + (K,), dtype=torch.float32 if float32 else BF16, device=codes.device)
+    with _device(codes):
+        call("moe_mx4_dequantize", ptr(codes), ptr(scales), out.numel() // K, K, int(float32), ptr(out),
+             _stream(codes), tag="mx4_dequantize")
+    return out
+
+
+@mx4_dequantize.register_fake
+def _(codes, scales, float32):
+    return codes.new_empty(codes.shape[:-1] + (2 * codes.shape[-1],), dtype=torch.float32 if float32 else BF16)
+
+
+def _check_mx4_product(what, a_codes, a_scales, w_codes, w_scales, offsets) -> tuple[int, int, int, int]:
+    """(rows, groups, weight rows, K)."""
+    if a_codes.dim() != 2 or w_codes.dim() != 3:
+        raise ValueError(f"{what}: activations must be [rows, K] and weights [groups, N, K], got codes "
+                         f"{tuple(a_codes.shape)} and {tuple(w_codes.shape)}")
+    K = _check_mx4(f"{what} activations", a_codes, a_scales)
+    if _check_mx4(f"{what} weights", w_codes, w_scales) != K:
+        raise ValueError(f"{what}: activations have {K} values a row, weights {2 * w_codes.shape[-1]}")
+    if offsets.dtype != torch.int32 or offsets.shape != (w_codes.shape[0],):
+        raise ValueError(f"{what}: offsets must be int32 [{w_codes.shape[0]}] (each group's end row), got "
+                         f"{offsets.dtype} {tuple(offsets.shape)}")
+    _require_gpu(a_codes, a_scales, w_codes, w_scales, offsets)
+    _require_one_device(a_codes, a_scales, w_codes, w_scales, offsets)
+    return a_codes.shape[0], w_codes.shape[0], w_codes.shape[1], K
+
+
+@_op("mx4_grouped_mm")
+def mx4_grouped_mm(a_codes: Tensor, a_scales: Tensor, w_codes: Tensor, w_scales: Tensor, offsets: Tensor) -> Tensor:
+    """[M, N] bf16: the rows of group g (up to offsets[g]) times W[g]^T; rows past the last group are not written."""
+    M, G, N, K = _check_mx4_product("mx4_grouped_mm", a_codes, a_scales, w_codes, w_scales, offsets)
+    a_codes, a_scales, w_codes, w_scales, offsets = map(_rows16, (a_codes, a_scales, w_codes, w_scales, offsets))
+    out = torch.empty(M, N, dtype=BF16, device=a_codes.device)
+    with _device(out):
+        call("moe_mx4_grouped_gemm", ptr(a_codes), ptr(a_scales), M, None, 1, ptr(w_codes), ptr(w_scales),
+             ptr(offsets), G, M, N, K, ptr(out), _stream(out), tag="mx4_down")
+    return out
+
+
+@mx4_grouped_mm.register_fake
+def _(a_codes, a_scales, w_codes, w_scales, offsets):
+    return a_codes.new_empty(a_codes.shape[0], w_codes.shape[1], dtype=BF16)
+
+
+@_op("mx4_grouped_swiglu")
+def mx4_grouped_swiglu(a_codes: Tensor, a_scales: Tensor, w_codes: Tensor, w_scales: Tensor,
+                       offsets: Tensor) -> Tensor:
+    """[M, I] bf16: silu(gate) * up of the rows of group g times W[g]^T, W [G, 2I, K] with the gate's rows first;
+    rows past the last group are not written."""
+    M, G, I2, K = _check_mx4_product("mx4_grouped_swiglu", a_codes, a_scales, w_codes, w_scales, offsets)
+    if I2 % 2:
+        raise ValueError(f"mx4_grouped_swiglu: {I2} weight rows are no gate and up halves")
+    a_codes, a_scales, w_codes, w_scales, offsets = map(_rows16, (a_codes, a_scales, w_codes, w_scales, offsets))
+    out = torch.empty(M, I2 // 2, dtype=BF16, device=a_codes.device)
+    with _device(out):
+        call("moe_mx4_grouped_swiglu", ptr(a_codes), ptr(a_scales), M, None, 1, ptr(w_codes), ptr(w_scales),
+             ptr(offsets), G, M, I2 // 2, K, ptr(out), None, None, _stream(out), tag="mx4_up")
+    return out
+
+
+@mx4_grouped_swiglu.register_fake
+def _(a_codes, a_scales, w_codes, w_scales, offsets):
+    return a_codes.new_empty(a_codes.shape[0], w_codes.shape[1] // 2, dtype=BF16)
+
+
+def _check_mx4_experts(hidden, top_k_index, top_k_weights, gu_codes, gu_scales, dn_codes, dn_scales):
+    if hidden.dim() != 2 or hidden.dtype not in (BF16, torch.float32):
+        raise ValueError(f"hidden states must be [tokens, hidden] bfloat16 or float32, got {tuple(hidden.shape)} "
+                         f"{hidden.dtype}")
+    if top_k_index.shape != top_k_weights.shape or top_k_index.dim() != 2 or top_k_index.shape[0] != hidden.shape[0]:
+        raise ValueError("top_k_index and top_k_weights must both be [tokens, k]")
+    if gu_codes.dim() != 3 or dn_codes.dim() != 3:
+        raise ValueError("expert weights must be [experts, rows, values]")
+    H, I = _check_mx4("gate_up_proj", gu_codes, gu_scales), _check_mx4("down_proj", dn_codes, dn_scales)
+    E = gu_codes.shape[0]
+    if hidden.shape[1] != H or gu_codes.shape[1] != 2 * I or tuple(dn_codes.shape[:2]) != (E, H):
+        raise ValueError(f"expert weights do not match: gate_up_proj ({E}, {gu_codes.shape[1]}, {H}), down_proj "
+                         f"({dn_codes.shape[0]}, {dn_codes.shape[1]}, {I}), hidden {hidden.shape[1]}")
+    tensors = (hidden, top_k_index, top_k_weights, gu_codes, gu_scales, dn_codes, dn_scales)
+    _require_gpu(*tensors)
+    _require_one_device(*tensors)
+    return hidden.shape[0], H, top_k_index.shape[1], E, I
+
+
+@_op("mx4_experts")
+def mx4_experts(hidden: Tensor, top_k_index: Tensor, top_k_weights: Tensor, gate_up_codes: Tensor,
+                gate_up_scales: Tensor, down_codes: Tensor, down_scales: Tensor) -> Tensor:
+    """experts_fwd on 4-bit weights: the tokens are quantised once, the sorted slots read them through the sort's
+    order, the act values are quantised as they are formed, and the combine sums bf16 rows in fp32."""
+    T, H, k, E, I = _check_mx4_experts(hidden, top_k_index, top_k_weights, gate_up_codes, gate_up_scales, down_codes,
+                                       down_scales)
+    S = T * k
+    dev = hidden.device
+    out = torch.empty(T, H, dtype=BF16, device=dev)
+    if S == 0:
+        return out.zero_().to(hidden.dtype)
+    ids, w = _ids64(top_k_index), top_k_weights.float().contiguous()
+    weights = tuple(map(_rows16, (gate_up_codes, gate_up_scales, down_codes, down_scales)))
+    u8 = dict(dtype=torch.uint8, device=dev)
+    x = _rows16(hidden)
+    with _device(hidden):
+        s = _stream(hidden)
+        perm, pos = torch.empty(2, S, dtype=torch.int32, device=dev).unbind()
+        counts, offsets = torch.empty(2, E, dtype=torch.int32, device=dev).unbind()
+        ws = _ws(_lib.load().moe_permute_workspace_bytes(S, E), dev)
+        call("moe_permute_fwd", None, T, 0, ptr(ids), k, 1, E, None, ptr(perm), ptr(pos), ptr(counts), ptr(offsets),
+             ptr(ws), ws.numel(), s, tag="permute_fwd")
+        xc, xs = torch.empty(T, H // 2, **u8), torch.empty(T, mx4_pitch(H), **u8)
+        call("moe_mx4_quantize", ptr(x), int(x.dtype == torch.float32), T, H, ptr(xc), ptr(xs), s, tag="mx4_quantize")
+        ac, asc = torch.empty(S, I // 2, **u8), torch.empty(S, mx4_pitch(I), **u8)
+        call("moe_mx4_grouped_swiglu", ptr(xc), ptr(xs), T, ptr(perm), k, ptr(weights[0]), ptr(weights[1]),
+             ptr(offsets), E, S, I, H, None, ptr(ac), ptr(asc), s, tag="mx4_up")
+        y = torch.empty(S, H, dtype=BF16, device=dev)
+        call("moe_mx4_grouped_gemm", ptr(ac), ptr(asc), S, None, 1, ptr(weights[2]), ptr(weights[3]), ptr(offsets), E,
+             S, H, I, ptr(y), s, tag="mx4_down")
+        call("moe_combine_fwd", ptr(y), ptr(pos), ptr(offsets), E, ptr(w), T, H, k, ptr(out), s, tag="combine_fwd")
+    return out.to(hidden.dtype)
+
+
+@mx4_experts.register_fake
+def _(hidden, top_k_index, top_k_weights, gate_up_codes, gate_up_scales, down_codes, down_scales):
+    return torch.empty_like(hidden)
+
+
+def run_mx4(name: str, *args):
+    """An mx4 op on tensors, with its refusal of gradients."""
+    _refuse_gradients(name, *args)
+    return _direct(name, *args)
 
 
 # ------------------------------------------------------------------ permute

@@ -1,0 +1,388 @@
+"""4-bit microscaled operands on the GPU: quantisation, the grouped products and the experts on them, against float64.
+
+Codes, scales and their values must be equal.  The products' bounds are counted in mx4_oracle: fp32 accumulation,
+then half a step of the bf16 output (2^-8); where act values are quantised on the way, a value that accumulation may
+carry over a rounding border may take the neighbouring code, and counts with that distance.
+"""
+
+import pytest
+import torch
+
+import mx4_oracle as O
+from parallel_amd import (
+    MX4Experts,
+    MX4Tensor,
+    MoeConfig,
+    SparseMoeBlock,
+    mx4_experts,
+    mx4_grouped_mm,
+    mx4_swiglu,
+    ops,
+    quantize_mx4,
+    residual_norm,
+)
+from parallel_amd._lib import call
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF = torch.bfloat16
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def pitch(K):
+    return 8 * -(-K // 256)
+
+
+def assert_quantized(x):
+    q = quantize_mx4(x)
+    idx, s = O.quantize(x)
+    K = x.shape[-1]
+    assert q.shape == x.shape and q.scales.shape == x.shape[:-1] + (pitch(K),)
+    assert torch.equal(q.block_scales, s)
+    assert torch.equal(q.codes, O.pack(idx))
+    assert not q.scales[..., K // 32:].any()
+    for dt in (torch.float32, BF):
+        assert torch.equal(torch.nan_to_num(q.dequantize(dt).double(), nan=1e300),
+                           torch.nan_to_num(O.values(idx, s).to(dt).double(), nan=1e300))
+    return q
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("shape", [(1, 32), (3, 96), (7, 256), (5, 288), (2, 3, 640), (33, 2048), (1000, 160), (32,)])
+def test_quantize_random(shape, dtype):
+    g = gen(sum(shape))
+    x = torch.randn(*shape, generator=g, device=DEV) * torch.exp(3 * torch.randn(*shape[:-1], 1, generator=g, device=DEV))
+    assert_quantized(x.to(dtype))
+
+
+def test_quantize_every_finite_bf16_value():
+    """Every bf16 value in a block that its own size rules, and in one whose scale is up to 2^4 larger."""
+    bits = torch.arange(65536, device=DEV, dtype=torch.int32).to(torch.int16)
+    x = bits.view(BF)
+    x = x[torch.isfinite(x)]
+    own = x.view(-1, 1).expand(-1, 32).contiguous()
+    assert_quantized(own)
+    for up in (2.0, 4.0, 16.0):
+        block = own.clone()
+        block[:, 7] = (own[:, 7].double().abs() * up).clamp(max=3e38).to(BF)
+        assert_quantized(block)
+
+
+def test_quantize_at_rounding_borders():
+    """fp32 values on and next to the middles between levels, at scales from the smallest to the largest."""
+    mid = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0], dtype=torch.float64, device=DEV)
+    for e in (-127, -126, -100, -1, 0, 1, 60, 125):
+        m = (mid * 2.0 ** e).float()
+        if e > -120:  # neighbours; subnormal ones below that keep the borders themselves
+            m = torch.cat((m, torch.nextafter(m, torch.full_like(m, 3e38)), torch.nextafter(m, -m)))
+        x = torch.zeros(m.numel(), 32, device=DEV)
+        x[:, 3] = 2.0 ** min(e + 2, 127)
+        x[:, 5], x[:, 30] = m, -m
+        assert_quantized(x)
+
+
+def test_quantize_special_blocks():
+    x = torch.randn(6, 96, generator=gen(3), device=DEV)
+    x[0, 40], x[1, 64], x[2, 0] = float("nan"), float("inf"), -float("inf")
+    x[3] = 0.0
+    x[4, 32:64] = -0.0
+    x[5, :32] = 3.4e38
+    for dt in (torch.float32, BF):
+        q = assert_quantized(x.to(dt))
+        assert q.block_scales[0].tolist()[1] == 255 and torch.isnan(q.dequantize()[0, 32:64]).all()
+        assert torch.isfinite(q.dequantize()[0, :32]).all()
+    assert_quantized(torch.full((2, 32), 1e-45, device=DEV))  # fp32 subnormals
+    assert quantize_mx4(torch.empty(0, 64, device=DEV)).dequantize().shape == (0, 64)
+
+
+def test_every_code_at_every_scale_dequantizes_exactly():
+    codes = torch.arange(256, device=DEV, dtype=torch.int32).to(torch.uint8).view(256, 1).expand(256, 16).contiguous()
+    codes = torch.cat((codes[:128], codes[128:]), dim=1)  # [128, 32]: two blocks a row
+    for s in range(256):
+        scales = torch.zeros(128, 8, dtype=torch.uint8, device=DEV)
+        scales[:, 0], scales[:, 1] = s, 255 - s
+        t = MX4Tensor(codes, scales)
+        want = O.values(O.unpack(codes), scales)
+        for dt in (torch.float32, BF):
+            got = t.dequantize(dt)
+            assert torch.equal(torch.isnan(got), torch.isnan(want)), s
+            assert torch.equal(torch.nan_to_num(got.double(), nan=0.0, posinf=1e300, neginf=-1e300),
+                               torch.nan_to_num(want.to(dt).double(), nan=0.0, posinf=1e300, neginf=-1e300)), s
+
+
+def operand(g, *shape, std=1.0):
+    """(MX4Tensor, its float64 values) of random codes from normal data."""
+    x = torch.randn(*shape, generator=g, device=DEV) * std
+    x = x * torch.exp(0.7 * torch.randn(*shape[:-2], 1, shape[-1], generator=g, device=DEV))
+    idx, s = O.quantize(x)
+    scales = torch.full(shape[:-1] + (pitch(shape[-1]),), 255, dtype=torch.uint8, device=DEV)  # padding is never read as NaN
+    scales[..., :s.shape[-1]] = s
+    return MX4Tensor(O.pack(idx), scales), O.values(idx, s)
+
+
+def within(got, want, err, what=""):
+    bound = want.abs() * 2.0 ** -8 + err * (1 + 2.0 ** -8) + 1e-38
+    off = (got.double() - want).abs()
+    worst = float((off / bound).max()) if off.numel() else 0.0
+    assert worst <= 1.0, f"{what}: {worst:.2f} of the bound"
+
+
+def offsets_of(counts):
+    return torch.tensor(counts, dtype=torch.int32, device=DEV).cumsum(0, dtype=torch.int32)
+
+
+COUNTS = [
+    [1], [0, 3], [5, 0, 0, 1], [16, 17], [1] * 40, [63, 64, 65, 0], [130, 2, 0, 33], [0] * 70 + [9] + [0] * 20 + [1],
+    [300, 129], [256, 257, 511], [1100],
+]
+
+
+@pytest.mark.parametrize("counts", COUNTS, ids=lambda c: f"{len(c)}x{sum(c)}")
+@pytest.mark.parametrize("N,K", [(8, 32), (40, 96), (200, 544), (264, 2080)])
+def test_grouped_products(counts, N, K):
+    g = gen(N + K + sum(counts))
+    a, av = operand(g, sum(counts), K)
+    w, wv = operand(g, len(counts), 2 * N, K, std=0.1)
+    offs = offsets_of(counts)
+    want, err = O.product(av, wv, counts)
+    within(mx4_grouped_mm(a, w, offs), want, err, "mm")
+    act, e = O.swiglu(want, err)
+    within(mx4_swiglu(a, w, offs), act, e, "swiglu")
+
+
+@pytest.mark.parametrize("rows,G,N,K", [(3000, 8, 512, 768), (700, 3, 768, 1024), (9000, 64, 256, 256), (130, 128, 96, 1536)])
+def test_larger_products(rows, G, N, K):
+    g = gen(rows)
+    counts = torch.bincount(torch.randint(G, (rows,), generator=g, device=DEV), minlength=G).tolist()
+    a, av = operand(g, rows, K)
+    w, wv = operand(g, G, 2 * N, K, std=0.1)
+    want, err = O.product(av, wv, counts)
+    within(mx4_grouped_mm(a, w, offsets_of(counts)), want, err, "mm")
+    within(mx4_swiglu(a, w, offsets_of(counts)), *O.swiglu(want, err), "swiglu")
+
+
+def test_nan_blocks_reach_their_rows_and_columns_alone():
+    g = gen(8)
+    counts = [20, 0, 50]
+    a, av = operand(g, 70, 320)
+    w, wv = operand(g, 3, 48, 320)
+    a.scales[33, 4] = 255
+    w.scales[0, 5, 9] = 255
+    av[33, 128:160] = float("nan")
+    wv[0, 5, 288:] = float("nan")
+    got = mx4_grouped_mm(a, w, offsets_of(counts))
+    want, _ = O.product(av, wv, counts)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert bool(torch.isnan(want[33]).all()) and int(torch.isnan(want).sum()) == 48 + 20 - 0
+
+
+@pytest.mark.parametrize("rows,counts", [(50, [10, 0, 20]), (600, [100, 257]), (40, [0, 0, 0]), (9, [0, 9])])
+def test_rows_behind_the_last_group_are_left_as_they_were(rows, counts):
+    g = gen(rows)
+    G, N, K, used = len(counts), 72, 288, sum(counts)
+    a, av = operand(g, rows, K)
+    w, wv = operand(g, G, 2 * N, K)
+    offs = offsets_of(counts)
+    s = torch.cuda.current_stream().cuda_stream
+    c = torch.full((rows, 2 * N), 7.0, dtype=BF, device=DEV)
+    call("moe_mx4_grouped_gemm", a.codes.data_ptr(), a.scales.data_ptr(), rows, None, 1, w.codes.data_ptr(),
+         w.scales.data_ptr(), offs.data_ptr(), G, rows, 2 * N, K, c.data_ptr(), s)
+    want, err = O.product(av[:used], wv, counts)
+    within(c[:used], want, err)
+    assert bool((c[used:] == 7.0).all())
+    w32, wv32 = operand(g, G, 64, K)
+    codes = torch.full((rows, 16), 0x5a, dtype=torch.uint8, device=DEV)
+    scales = torch.full((rows, 8), 0x33, dtype=torch.uint8, device=DEV)
+    call("moe_mx4_grouped_swiglu", a.codes.data_ptr(), a.scales.data_ptr(), rows, None, 1, w32.codes.data_ptr(),
+         w32.scales.data_ptr(), offs.data_ptr(), G, rows, 32, K, None, codes.data_ptr(), scales.data_ptr(), s)
+    act, e = O.swiglu(*O.product(av[:used], wv32, counts))
+    mid, far = O.requantize(act, e)
+    assert bool(((O.values(O.unpack(codes[:used]), scales[:used]) - mid).abs() <= far).all())
+    assert bool((codes[used:] == 0x5a).all()) and bool((scales[used:] == 0x33).all())
+
+
+def layer(g, E, H, I):
+    gu, guv = operand(g, E, 2 * I, H, std=H ** -0.5)
+    dn, dnv = operand(g, E, H, I, std=I ** -0.5)
+    return gu, guv, dn, dnv
+
+
+def experts_oracle(x, idx, wts, guv, dnv):
+    """(out, bound) of the path: quantised tokens, fp32 products, quantised act, bf16 rows, fp32 combine."""
+    E = guv.shape[0]
+    xv = O.values(*O.quantize(x))
+    T, k = idx.shape
+    out, err = torch.zeros(T, x.shape[1], dtype=torch.float64, device=DEV), None
+    err, size = torch.zeros_like(out), torch.zeros_like(out)
+    for e in range(E):
+        t, j = (idx == e).nonzero(as_tuple=True)
+        if not t.numel():
+            continue
+        act, ea = O.swiglu(*O.product(xv[t], guv[e:e + 1], [t.numel()]))
+        mid, far = O.requantize(act, ea)
+        y, ey = O.product(mid, dnv[e:e + 1], [t.numel()])
+        ey = ey + far @ dnv[e].t().abs()
+        ey = ey + 2.0 ** -8 * (y.abs() + ey)  # the rows are held in bf16
+        wt = wts[t, j].double().unsqueeze(1)
+        out.index_add_(0, t, wt * y)
+        err.index_add_(0, t, wt.abs() * ey)
+        size.index_add_(0, t, (wt * y).abs())
+    return out, err + 2 * k * O.U * (size + err)
+
+
+@pytest.mark.parametrize("T,H,E,k,I", [(1, 64, 8, 2, 32), (1, 2048, 128, 8, 768), (7, 256, 8, 2, 128), (48, 512, 32, 4, 160),
+                                       (333, 416, 8, 3, 288), (1500, 512, 4, 2, 256), (4096, 256, 16, 2, 96)])
+def test_experts(T, H, E, k, I):
+    g = gen(T + H)
+    gu, guv, dn, dnv = layer(g, E, H, I)
+    x = (torch.randn(T, H, generator=g, device=DEV) * 2).to(BF)
+    top = torch.topk(torch.randn(T, E, generator=g, device=DEV), k, dim=1)
+    wts = torch.softmax(top.values, 1)
+    within(mx4_experts(x, top.indices, wts, gu, dn), *experts_oracle(x, top.indices, wts, guv, dnv))
+
+
+def test_experts_routing_corners():
+    """Sentinel ids, a token without any expert, the same expert twice for a token, all tokens on one expert,
+    weights of zero, fp32 hidden states, int32 ids."""
+    g = gen(4)
+    E, H, I, T = 8, 128, 64, 70
+    gu, guv, dn, dnv = layer(g, E, H, I)
+    x = torch.randn(T, H, generator=g, device=DEV)
+    idx = torch.full((T, 3), 5, device=DEV)
+    idx[10:30, 0] = E  # the sentinel
+    idx[20, :] = E
+    idx[40:, 1] = torch.randint(E, (30,), generator=g, device=DEV)
+    wts = torch.rand(T, 3, generator=g, device=DEV)
+    wts[3] = 0.0
+    for dt in (torch.float32, BF):
+        out = mx4_experts(x.to(dt), idx.int(), wts, gu, dn)
+        assert out.dtype == dt
+        within(out, *experts_oracle(x.to(dt), idx, wts, guv, dnv))
+        assert not out[20].any() and not out[3].any()
+    x[6, 17] = float("inf")
+    bad = mx4_experts(x, idx, wts, gu, dn)
+    assert torch.isnan(bad[6]).all() and torch.isfinite(bad[torch.arange(T, device=DEV) != 6]).all()
+    assert mx4_experts(x[:0], idx[:0], wts[:0], gu, dn).shape == (0, H)
+
+
+def test_strided_and_misaligned_operands():
+    g = gen(12)
+    a, _ = operand(g, 40, 256)
+    w, _ = operand(g, 2, 64, 256)
+    offs = offsets_of([13, 27])
+    want = mx4_grouped_mm(a, w, offs)
+    codes = torch.empty(40 * 128 + 1, dtype=torch.uint8, device=DEV)[1:].view(40, 128).copy_(a.codes)
+    scales = torch.empty(40, 24, dtype=torch.uint8, device=DEV)[:, 3:11].copy_(a.scales)
+    turned = MX4Tensor(w.codes.transpose(0, 1).contiguous().transpose(0, 1), w.scales.flip(0).flip(0))
+    every_other = torch.stack((offs, offs), 1).reshape(-1)[::2]
+    assert torch.equal(mx4_grouped_mm(MX4Tensor(codes, scales), turned, every_other), want)
+    x = torch.randn(256, 64, generator=g, device=DEV).to(BF)
+    assert torch.equal(quantize_mx4(x.t()).codes, quantize_mx4(x.t().contiguous()).codes)
+    unpadded = MX4Tensor(a.codes[:, :48].contiguous(), a.scales[:, :3].contiguous())  # K = 96: 3 bytes a row given
+    assert unpadded.scales.shape == (40, 8) and unpadded.shape == (40, 96)
+
+
+def test_replays_of_a_captured_layer_and_another_stream():
+    g = gen(21)
+    E, H, I, T = 16, 256, 128, 37
+    gu, _, dn, _ = layer(g, E, H, I)
+    x = torch.randn(T, H, generator=g, device=DEV).to(BF)
+    top = torch.topk(torch.randn(T, E, generator=g, device=DEV), 4, dim=1)
+    idx, wts = top.indices.clone(), torch.softmax(top.values, 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = mx4_experts(x, idx, wts, gu, dn)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, mx4_experts(x, idx, wts, gu, dn))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = mx4_experts(x, idx, wts, gu, dn)
+    for n in range(3):
+        x.copy_(torch.randn(T, H, generator=g, device=DEV))
+        idx.copy_(torch.topk(torch.randn(T, E, generator=g, device=DEV), 4, dim=1).indices)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, mx4_experts(x, idx, wts, gu, dn)), n
+
+
+def test_modules_run_together_between_two_blocks():
+    """Residual norm, router, experts on 4-bit weights, residual norm: the layer's second half as inference runs it."""
+    g = gen(30)
+    cfg = MoeConfig(hidden_size=256, num_experts=16, num_experts_per_tok=4, moe_intermediate_size=96, norm_topk_prob=True)
+    block = SparseMoeBlock(cfg).to(DEV, BF)
+    with torch.no_grad():
+        for p in block.parameters():
+            p.copy_(torch.randn(p.shape, generator=g, device=DEV) * 0.06)
+        block.experts = MX4Experts.from_experts(block.experts)
+        attn, stream = (torch.randn(2, 45, 256, generator=g, device=DEV).to(BF) for _ in range(2))
+        n1, n2 = (1 + 0.1 * torch.randn(256, generator=g, device=DEV).to(BF) for _ in range(2))
+        hidden, x = residual_norm(attn, stream, n1)
+        moe = block(x)
+        out, nxt = residual_norm(moe, hidden, n2)
+        _, scores, idx = block.gate(x.view(-1, 256))
+    ex = block.experts
+    values = [O.values(O.unpack(c), s) for c, s in ((ex.gate_up_codes, ex.gate_up_scales), (ex.down_codes, ex.down_scales))]
+    within(moe.view(-1, 256), *experts_oracle(x.view(-1, 256), idx, scores, *values), "experts")
+    h = hidden.double() + moe.double()
+    assert bool(((out.double() - h).abs() <= h.abs() * 2.0 ** -8 + 4 * O.U * (hidden.double().abs() + moe.double().abs())).all())
+    want = h * (h.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * n2.double()
+    assert bool(((nxt.double() - want).abs() <= want.abs() * (2.0 ** -8 + 64 * O.U) + 1e-6).all())
+    state = block.state_dict()
+    other = SparseMoeBlock(cfg).to(DEV, BF)
+    other.experts = MX4Experts(*(MX4Tensor(torch.zeros_like(c), torch.zeros_like(s))
+                                 for c, s in ((ex.gate_up_codes, ex.gate_up_scales), (ex.down_codes, ex.down_scales))))
+    other.load_state_dict(state)
+    with torch.no_grad():
+        assert torch.equal(other(x), moe)
+
+
+def test_a_transformers_block_takes_the_module():
+    modeling = pytest.importorskip("transformers.models.qwen3_moe.modeling_qwen3_moe")
+    from transformers import Qwen3MoeConfig
+
+    cfg = Qwen3MoeConfig(hidden_size=128, num_experts=8, num_experts_per_tok=2, moe_intermediate_size=64,
+                         norm_topk_prob=True)
+    block = modeling.Qwen3MoeSparseMoeBlock(cfg).to(DEV, BF)
+    g = gen(31)
+    with torch.no_grad():
+        for p in block.parameters():
+            p.copy_(torch.randn(p.shape, generator=g, device=DEV) * 0.1)
+        x = torch.randn(1, 20, 128, generator=g, device=DEV).to(BF)
+        block.experts = MX4Experts.from_experts(block.experts)
+        out = block(x)
+        out = out[0] if isinstance(out, tuple) else out
+        flat = x.view(-1, 128)
+        gate = block.gate(flat)
+        want = block.experts(flat, gate[2], gate[1])
+    assert torch.equal(out.view(-1, 128), want)
+
+
+def test_gradients_are_refused():
+    g = gen(1)
+    gu, _, dn, _ = layer(g, 4, 64, 32)
+    x = torch.randn(3, 64, generator=g, device=DEV).to(BF).requires_grad_()
+    idx = torch.zeros(3, 1, dtype=torch.int64, device=DEV)
+    for call_it in (lambda: quantize_mx4(x), lambda: mx4_experts(x, idx, torch.ones(3, 1, device=DEV), gu, dn)):
+        with pytest.raises(ValueError, match="no gradient"):
+            call_it()
+        with torch.no_grad():
+            call_it()
+
+
+def test_the_ops_pass_torch_library_checks():
+    g = gen(2)
+    gu, _, dn, _ = layer(g, 4, 64, 32)
+    x = torch.randn(5, 64, generator=g, device=DEV).to(BF)
+    idx = torch.randint(4, (5, 2), generator=g, device=DEV)
+    a = quantize_mx4(x)
+    offs = offsets_of([2, 0, 3, 0])
+    lib = torch.ops.parallel_amd
+    for op, args in ((lib.mx4_quantize, (x,)), (lib.mx4_dequantize, (a.codes, a.scales, True)),
+                     (lib.mx4_grouped_mm, (a.codes, a.scales, gu.codes, gu.scales, offs)),
+                     (lib.mx4_grouped_swiglu, (a.codes, a.scales, gu.codes, gu.scales, offs)),
+                     (lib.mx4_experts, (x, idx, torch.ones(5, 2, device=DEV), gu.codes, gu.scales, dn.codes, dn.scales))):
+        torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
