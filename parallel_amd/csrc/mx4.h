@@ -175,5 +175,7 @@ __device__ __forceinline__ void mx4_store_rows(const Mx4Gemm& p, const f32x4_t (
 
 // Products of few rows per group (mx4_few.hip).
 int mx4_few(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name);
+// Products of many rows per group in tiles of up to bm (64, 128 or 256) rows (mx4_tile.hip).
+int mx4_tile(const Mx4Gemm& p, int epi, int bm, hipStream_t stream, const char* name);
 
 }  // namespace moe

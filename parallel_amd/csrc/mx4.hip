@@ -161,7 +161,9 @@ int run_product(const char* what, const void* a, const void* a_scales, int64_t a
   p.c = static_cast<bf16_t*>(c);
   p.c_codes = static_cast<uint8_t*>(c_codes);
   p.c_scales = static_cast<uint8_t*>(c_scales);
-  return mx4_few(p, epi, as_stream(stream), what);
+  const int64_t mean = (M + G - 1) / G;
+  if (mean <= 32) return mx4_few(p, epi, as_stream(stream), what);
+  return mx4_tile(p, epi, mean <= 64 ? 64 : mean <= 128 ? 128 : 256, as_stream(stream), what);
 }
 }  // namespace
 
