@@ -26,11 +26,18 @@ __device__ __forceinline__ uint32_t mx4_scale(uint32_t top) {
 // exponent alone (also 0, for 2^-127).
 __device__ __forceinline__ float mx4_scale_f(uint32_t s) { return __uint_as_float(s << 23); }
 
+// silu(g) u with the hardware's exponential and reciprocal (1 ulp each).
+__device__ __forceinline__ float mx4_act(float g, float u) {
+  const float e = __builtin_amdgcn_exp2f(-1.44269504f * g);  // past the float range: 0 or infinity
+  return g * u * __builtin_amdgcn_rcpf(1.0f + e);
+}
+
 // One product launch.
 struct Mx4Gemm {
   const uint8_t *a, *a_scales;  // [a_rows, K]
   const int32_t* row_index;     // row r of the product reads row row_index[r] / row_div of A (null: row r)
   int row_div, a_rows;
+  uint32_t div_magic, div_shift;  // x / row_div = x * div_magic >> div_shift for 0 <= x < 2^31
   const uint8_t *w, *w_scales;  // [G][N, K], or with swiglu [G][2 N, K]: gate rows, then up rows
   const int32_t* offs;
   int G, rows, N, K;
@@ -48,6 +55,12 @@ __device__ __forceinline__ int mx4_group_rows(const Mx4Gemm& p, int g, int& lo) 
     lo = g ? min(max(p.offs[g - 1], 0), hi) : 0;
   }
   return hi - lo;
+}
+
+// The row of A behind entry i of row_index (negative entries stay out of range).
+__device__ __forceinline__ int mx4_source_row(const Mx4Gemm& p, int i) {
+  const uint64_t q = static_cast<uint64_t>(static_cast<uint32_t>(i)) * p.div_magic >> p.div_shift;
+  return i < 0 ? -1 : static_cast<int>(q);
 }
 
 struct Mx4Tile {
@@ -136,7 +149,7 @@ __device__ __forceinline__ void mx4_store_rows(const Mx4Gemm& p, const f32x4_t (
 #pragma unroll
     for (int j = 0; j < NT / 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) act[j][e] = silu_f(v[2 * j][e]) * v[2 * j + 1][e];
+      for (int e = 0; e < 4; ++e) act[j][e] = mx4_act(v[2 * j][e], v[2 * j + 1][e]);
     if constexpr (EPI == MX4_SWIGLU) {
 #pragma unroll
       for (int j = 0; j < NT / 2; ++j) {

@@ -150,6 +150,11 @@ int run_product(const char* what, const void* a, const void* a_scales, int64_t a
   p.a_scales = static_cast<const uint8_t*>(a_scales);
   p.row_index = row_index;
   p.row_div = static_cast<int>(row_div);
+  // Granlund and Montgomery's multiplier: with l = ceil(log2 d), m = floor(2^(31+l) / d) + 1 divides 31-bit numbers.
+  uint32_t l = 0;
+  while ((1ll << l) < row_div) ++l;
+  p.div_magic = static_cast<uint32_t>((1ull << (31 + l)) / static_cast<uint64_t>(row_div) + 1);
+  p.div_shift = 31 + l;
   p.a_rows = static_cast<int>(a_rows);
   p.w = static_cast<const uint8_t*>(w);
   p.w_scales = static_cast<const uint8_t*>(w_scales);

@@ -38,7 +38,7 @@ __global__ __launch_bounds__(WK * kWave) void mx4_few_kernel(const Mx4Gemm p, in
     const int m = 16 * i + i16;
     a_in[i] = m < t.rows;
     int r = t.r0 + (a_in[i] ? m : 0);
-    if (p.row_index) r = p.row_index[r] / p.row_div;
+    if (p.row_index) r = mx4_source_row(p, p.row_index[r]);
     a_in[i] = a_in[i] && r >= 0 && r < p.a_rows;
     a_row[i] = a_in[i] ? r : 0;
   }

@@ -1,22 +1,25 @@
 // Grouped products of mx4 operands for groups of many rows: LDS tiles of up to
-// BM rows by 256 weight rows (128 act columns with swiglu, gate and up in
-// 16-row turns), 256 values deep, so a row of a stage is one 128-byte line.
+// BM rows by 256 weight rows (128 act columns with swiglu, gate and up), 256
+// values deep, so a row of a stage is one 128-byte line.
 //
 // Eight waves, two by rows and four by columns; wave row wm owns the 16-row
 // tiles wm, wm + 2, ... (a partly filled tile then loads both), wave column wn
 // the 64 weight rows 64 wn ...  Products are v_mfma_scale_f32_16x16x128 on
 // codes and scales as they are stored: lane l multiplies the 32-blocks 2 (l /
 // 16) and + 1 of a stage's row, so its two codes chunks are neighbours and its
-// two scales one 16-bit read.
+// two scales one 16-bit read.  The scales come 16 bytes (two stages) of a row
+// at a time into a ring of their own: fetched stage by stage they were as many
+// L2 requests as the codes' whole lines.  The wave's 64 weight rows are dealt to its four
+// fragments four rows at a time, so that a lane's results are 16 neighbouring
+// output columns of one row (8 act columns with swiglu), stored as they are.
 //
 // Blocks are persistent, one per CU, and run one stream of stages over their
-// tiles: a DMA cursor (buffer_load ... lds) fills a ring of STAGES stages
-// STAGES - 1 ahead of the compute cursor and runs on across tiles, so that a
-// tile's first stage is on its way while the last one's output is written.
-// The epilogue turns each 16-row result into whole 16-byte pieces through the
-// stage just multiplied (which the DMA reaches a barrier later); it issues the
-// same number of stores whatever is in range (out of range ones are dropped by
-// the buffer resource), so that the waits that follow can leave them in flight.
+// tiles: a DMA cursor (buffer_load ... lds, fired between the products) fills a
+// ring of STAGES stages STAGES - 1 ahead of the compute cursor and runs on
+// across tiles, so that a tile's first stage is on its way while the last one's
+// output is written.  The epilogue issues the same number of stores whatever is
+// in range (out of range ones are dropped by the buffer resource), so that the
+// waits that follow can leave them in flight.
 #include "dma.h"
 #include "mx4.h"
 
@@ -25,35 +28,17 @@ namespace {
 
 constexpr int kTileWaves = 8, kTileThreads = kTileWaves * kWave;
 constexpr int kTileN = 256;     // weight rows per tile
-constexpr int kGroupRegs = 4;   // groups held in registers, 64 each
 constexpr int kXcds = 8;
 
-// 4 bytes per lane from `rsrc` + voffset into LDS at M0 + 4 lane (dma16 for scales).
-__device__ __forceinline__ void dma4(u32x4_t rsrc, uint32_t voffset, uint32_t lds_addr) {
-  asm volatile("s_nop 4\n\tbuffer_load_dword %0, %1, 0 offen lds" ::"v"(voffset), "s"(rsrc), "{m0}"(lds_addr)
-               : "memory");
+// f(first group, rows below it in its 64, lo, cnt) for every 64 groups, a group per lane.
+template <class F>
+__device__ __forceinline__ void each_groups(const Mx4Gemm& p, F&& f) {
+  for (int c0 = 0; c0 < p.G; c0 += kWave) {
+    int lo;
+    const int cnt = mx4_group_rows(p, c0 + (threadIdx.x & (kWave - 1)), lo);
+    f(c0, lo, cnt);
+  }
 }
-
-// The groups' first rows and counts, one group per lane and register.
-struct Groups {
-  int lo[kGroupRegs], cnt[kGroupRegs];
-  __device__ __forceinline__ void load(const Mx4Gemm& p) {
-#pragma unroll
-    for (int c = 0; c < kGroupRegs; ++c) cnt[c] = mx4_group_rows(p, c * kWave + (threadIdx.x & (kWave - 1)), lo[c]);
-  }
-  // f(first group, lo, cnt) for each 64 groups until it returns true.
-  template <class F>
-  __device__ __forceinline__ void each(const Mx4Gemm& p, F&& f) const {
-#pragma unroll
-    for (int c = 0; c < kGroupRegs; ++c)
-      if (c * kWave < p.G && f(c * kWave, lo[c], cnt[c])) return;
-    for (int c0 = kGroupRegs * kWave; c0 < p.G; c0 += kWave) {
-      int l;
-      const int n = mx4_group_rows(p, c0 + (threadIdx.x & (kWave - 1)), l);
-      if (f(c0, l, n)) return;
-    }
-  }
-};
 
 template <int BM, int STAGES, int EPI>
 __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p, int n_tiles) {
@@ -61,15 +46,16 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
   constexpr int WM = 2, MT = BM / 16 / WM, NT = 4;
   constexpr int kCols = GLU ? kTileN / 2 : kTileN;     // output columns per tile
   constexpr int LA = BM / 64, LB = kTileN / 64;        // code DMAs per wave and stage (8 rows each)
-  constexpr int LPW = LA + LB + 2;                     // and one for either operand's scales (32 rows each)
-  constexpr int kB = BM * 128, kAs = kB + kTileN * 128, kBs = kAs + BM * 8, kSpare = kBs + kTileN * 8;
-  constexpr int kStage = (kSpare + 256 + 1023) / 1024 * 1024;  // the spare 256 bytes take scale DMAs of rows past BM
-  constexpr int kStores = EPI == MX4_PLAIN ? 2 * MT : EPI == MX4_SWIGLU ? MT : 2 * ((MT * 16 + 63) / 64);
-  constexpr int kSlot = 16 * 144;                      // a wave's epilogue staging: 16 rows of 64 bf16, 16 bytes apart
-  static_assert(kTileWaves * kSlot <= kStage && MT * 16 * 17 <= kSlot, "the epilogue stages in one ring stage");
-  static_assert(STAGES * kStage <= 160 * 1024, "LDS");
+  constexpr int LPW = LA + LB;
+  constexpr int kB = BM * 128, kStage = kB + kTileN * 128;
+  constexpr int kScaleWaves = (BM + kTileN) / 64;      // waves that fetch scales, 64 rows each: A's, then B's
+  constexpr int kScales = kScaleWaves * 1024, kBs = BM * 16;
+  constexpr int kStores = EPI == MX4_SWIGLU ? MT : 2 * MT;  // store instructions per wave and tile
+  // 16-row tiles between whose products the next stage's DMA is fired: a ring of two needs it early.
+  constexpr int kFire = STAGES == 2 ? MT / 2 : MT;
+  static_assert(kScaleWaves <= kTileWaves && STAGES * (kStage + kScales) <= 160 * 1024, "LDS");
   static_assert((STAGES - 2) * LPW + kStores < 64, "vmcnt range");
-  __shared__ __attribute__((aligned(1024))) char ring[STAGES * kStage];
+  __shared__ __attribute__((aligned(1024))) char ring[STAGES * (kStage + kScales)];  // the stages, then their scales
 
   const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -78,12 +64,9 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
   const uint32_t half_k = static_cast<uint32_t>(p.K) / 2, pitch = static_cast<uint32_t>(mx4_pitch(p.K));
   const int blocks = p.K / 32, nk = (p.K + 255) / 256;
 
-  Groups groups;
-  groups.load(p);
   int total = 0;
-  groups.each(p, [&](int, int, int cnt) {
+  each_groups(p, [&](int, int, int cnt) {
     total += __builtin_amdgcn_readlane(wave_inclusive_scan((cnt + BM - 1) / BM), kWave - 1);
-    return false;
   });
   total = __builtin_amdgcn_readfirstlane(total) * n_tiles;
   // This block's tiles: every nbx-th of its XCD's contiguous share.
@@ -93,133 +76,156 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
   const int ntiles = span > xidx ? (span - xidx + nbx - 1) / nbx : 0;
   if (ntiles <= 0) return;  // the whole block
 
-  auto find = [&](int j) __attribute__((always_inline)) {  // tile j of the block's (j < ntiles)
-    Mx4Tile t{0, 0, 0, 0};
-    const int tile = first + j * nbx;
+  // Lane l holds the block's tile seen + l, so that a tile costs four lane
+  // reads; the lanes move on when a cursor passes them.
+  Mx4Tile held{0, 0, 0, 0};
+  int seen = 0;
+  auto hold = [&](int j0) __attribute__((always_inline)) {
+    seen = j0;
+    held = Mx4Tile{0, 0, 0, 0};
+    const int tile = first + (j0 + lane) * nbx;
+    const bool live = j0 + lane < ntiles;
     int base = 0;
-    groups.each(p, [&](int c0, int lo, int cnt) {
+    each_groups(p, [&](int c0, int lo, int cnt) {
       const int n = n_tiles * ((cnt + BM - 1) / BM);
       const int incl = wave_inclusive_scan(n);
       const int tot = __builtin_amdgcn_readlane(incl, kWave - 1);
-      if (tile >= base + tot) {
-        base += tot;
-        return false;
+      const int local = tile - base;
+      int w = 0;  // the first lane whose sum passes `local`
+#pragma unroll
+      for (int step = kWave / 2; step >= 1; step >>= 1)
+        if (__shfl(incl, w + step - 1) <= local) w += step;
+      const int rows = __shfl(cnt, w), start = __shfl(lo, w), before = __shfl(incl - n, w);
+      if (live && local >= 0 && local < tot) {
+        const int parts = (rows + BM - 1) / BM, per = ((rows + parts - 1) / parts + 15) & ~15;
+        const int nt = (local - before) / parts, part = local - before - nt * parts;
+        held = Mx4Tile{c0 + w, start + part * per, min(per, rows - part * per), nt};
       }
-      const int w = __builtin_amdgcn_readfirstlane(__builtin_ctzll(__ballot(base + incl > tile)));
-      const int local = tile - base - __builtin_amdgcn_readlane(incl - n, w);
-      const int rows = __builtin_amdgcn_readlane(cnt, w), parts = (rows + BM - 1) / BM;
-      const int per = ((rows + parts - 1) / parts + 15) & ~15;
-      const int nt = local / parts, part = local - nt * parts;
-      t = Mx4Tile{c0 + w, __builtin_amdgcn_readlane(lo, w) + part * per, min(per, rows - part * per), nt};
-      return true;
+      base += tot;
     });
-    t.g = __builtin_amdgcn_readfirstlane(t.g);
-    t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
-    t.rows = __builtin_amdgcn_readfirstlane(t.rows);
-    t.n = __builtin_amdgcn_readfirstlane(t.n);
-    return t;
+  };
+  auto find = [&](int j) __attribute__((always_inline)) {  // tile j of the block's, seen <= j < seen + 64
+    const int l = j - seen;
+    return Mx4Tile{__builtin_amdgcn_readlane(held.g, l), __builtin_amdgcn_readlane(held.r0, l),
+                   __builtin_amdgcn_readlane(held.rows, l), __builtin_amdgcn_readlane(held.n, l)};
   };
 
   // ------------------------------------------------------------ DMA cursor
   // Code DMA j of a wave fills rows 8 (wave L + j) .. + 7 of an operand, lane l
-  // the 16-byte slot l % 8 of row l / 8; slot s of row r holds chunk s ^ ((r /
-  // 2) % 8), so that the 16 rows of a fragment read lie on distinct banks.
-  // The scale DMA of a wave fills rows 32 wave .. + 31, lane l half l % 2 of row l / 2.
+  // the 16-byte slot l % 8 of row l / 8; chunk 2 q + s of row r is at slot
+  // (4 s + q) ^ key(r).  A pass of ds_read_b128 takes rows 0-3 and 12-15 of one
+  // lane quarter with rows 4-11 of the next: with chunk numbers that differ by
+  // one between quarters and the eight keys of a fragment's row pairs (a_key of
+  // neighbouring rows, b_key of rows 16 a + 4 j + b) its lanes lie on distinct
+  // banks.
+  // Every second stage, wave w's scale DMA takes 16 bytes of each of 64 rows: of
+  // A rows 64 w + lane, or behind them of B the rows of wave column w - BM / 64,
+  // fragment by fragment (position 16 j + 4 a + b: row 16 a + 4 j + b).
   const uint32_t lds0 = lds_address(ring);
   const u32x4_t ra = rsrc_words(p.a, static_cast<uint32_t>(p.a_rows) * half_k);
   const u32x4_t ras = rsrc_words(p.a_scales, static_cast<uint32_t>(p.a_rows) * pitch);
-  u32x4_t rb = ra, rbs = ra;
-  uint32_t a_off[LA], b_off[LB], as_off, bs_off;  // at stage 0; kOOB for rows past the end
-  int next_row[LA + 1];  // the source rows of the tile behind the cursor's (gathered activations), -1 past its end
+  u32x4_t rb = ra, rs = ra;
+  uint32_t a_off[LA], b_off[LB], s_off;  // at stage 0; kOOB for rows past the end
+  int next_row[LA + 1], next_rows = 0;  // of the tile behind the cursor's: its entries of row_index, its rows
   const int l8 = lane >> 3, slot = lane & 7;
-  auto chunk_of = [&](int r) { return static_cast<uint32_t>(slot ^ ((r >> 1) & 7)); };
-  auto tile_row = [&](int j) { return j < LA ? 8 * (wave * LA + j) + l8 : 32 * wave + (lane >> 1); };
-  int dj = -1, dk = nk;
+  auto a_key = [](int r) { return (r >> 1) & 7; };
+  auto b_key = [](int r) { return ((r >> 1) & 1) | ((r >> 4) & 3) << 1; };
+  auto chunk_at = [&](int key) { return ((slot ^ key) & 3) << 1 | (slot ^ key) >> 2; };
+  auto a_chunk = [&](int j) { return chunk_at(a_key(8 * (wave * LA + j) + l8)); };
+  auto b_chunk = [&](int j) { return chunk_at(b_key(8 * (wave * LB + j) + l8)); };
+  auto tile_row = [&](int j) { return j < LA ? 8 * (wave * LA + j) + l8 : 64 * wave + lane; };
+  int cj = 0, dj = -1, dk = nk;  // the compute cursor's tile; the DMA cursor's tile and stage
   auto fetch_rows = [&](int j) __attribute__((always_inline)) {
-    Mx4Tile t{0, 0, 0, 0};
-    if (j < ntiles) t = find(j);
+    if (j - seen >= kWave) hold(cj);  // (the DMA cursor is a few tiles ahead at most)
+    const Mx4Tile t = find(j);        // past the last tile: no rows
+    next_rows = t.rows;
 #pragma unroll
-    for (int n = 0; n <= LA; ++n) {
-      const int r = tile_row(n);
-      next_row[n] = r < t.rows ? t.r0 + r : -1;
-      if (p.row_index && r < t.rows) next_row[n] = p.row_index[t.r0 + r] / p.row_div;
+    for (int n = 0; n <= LA; ++n) next_row[n] = min(t.r0 + tile_row(n), p.rows - 1);
+    if (p.row_index) {
+#pragma unroll
+      for (int n = 0; n <= LA; ++n) next_row[n] = p.row_index[next_row[n]];
     }
   };
   auto seek = [&]() __attribute__((always_inline)) {  // to the next tile's first stage
     ++dj;
     dk = 0;
     const bool live = dj < ntiles;
-    Mx4Tile t{0, 0, 0, 0};
-    if (live) t = find(dj);
-    auto source = [&](int n) { return next_row[n] >= 0 && next_row[n] < p.a_rows; };
-#pragma unroll
-    for (int j = 0; j < LA; ++j)
-      a_off[j] = source(j) ? static_cast<uint32_t>(next_row[j]) * half_k + 16u * chunk_of(tile_row(j)) : kOOB;
-    as_off = source(LA) ? static_cast<uint32_t>(next_row[LA]) * pitch + 4u * (lane & 1) : kOOB;
-    auto weight_row = [&](int r, bool& in) {
-      const int n = t.n * kCols + (GLU ? (r >> 5) * 16 + (r & 15) : r);
-      in = live && n < p.N;
-      return static_cast<uint32_t>(GLU && (r & 16) ? p.N + n : n);
+    const Mx4Tile t = find(dj);
+    auto source = [&](int n, uint32_t row_bytes, uint32_t off) {
+      const int r = p.row_index ? mx4_source_row(p, next_row[n]) : next_row[n];
+      return tile_row(n) < next_rows && r >= 0 && r < p.a_rows ? static_cast<uint32_t>(r) * row_bytes + off : kOOB;
     };
-    bool in;
 #pragma unroll
-    for (int j = 0; j < LB; ++j) {
-      const int r = 8 * (wave * LB + j) + l8;
-      const uint32_t w = weight_row(r, in);
-      b_off[j] = in ? w * half_k + 16u * chunk_of(r) : kOOB;
-    }
-    const uint32_t w = weight_row(32 * wave + (lane >> 1), in);
-    bs_off = in ? w * pitch + 4u * (lane & 1) : kOOB;
+    for (int j = 0; j < LA; ++j) a_off[j] = source(j, half_k, 16u * a_chunk(j));
+    auto weight = [&](int r, uint32_t row_bytes, uint32_t off) {  // row r of the tile's: fragment (r / 4) % 4
+      const int j = (r >> 2) & 3;
+      const int n = t.n * kCols + (GLU ? (r >> 6) * 32 + ((r >> 4) & 3) * 8 + (j >> 1) * 4 + (r & 3) : r);
+      const int w = GLU && (j & 1) ? p.N + n : n;
+      return live && n < p.N ? static_cast<uint32_t>(w) * row_bytes + off : kOOB;
+    };
+#pragma unroll
+    for (int j = 0; j < LB; ++j) b_off[j] = weight(8 * (wave * LB + j) + l8, half_k, 16u * b_chunk(j));
     rb = rsrc_words(p.w + t.g * wide * half_k, static_cast<uint32_t>(wide) * half_k);
-    rbs = rsrc_words(p.w_scales + t.g * wide * pitch, static_cast<uint32_t>(wide) * pitch);
+    if (wave < BM / 64) {
+      s_off = source(LA, pitch, 0);
+      rs = ras;
+    } else {
+      s_off = weight(64 * (wave - BM / 64) + ((lane >> 2) & 3) * 16 + (lane >> 4) * 4 + (lane & 3), pitch, 0);
+      rs = rsrc_words(p.w_scales + t.g * wide * pitch, static_cast<uint32_t>(wide) * pitch);
+    }
     fetch_rows(dj + 1);
   };
-  auto issue = [&](int stage) __attribute__((always_inline)) {  // the cursor's stage into the ring, and on
-    const uint32_t at = lds0 + stage * kStage;
-    const uint32_t ahead = 128u * dk;
-    auto chunk_in = [&](int r) { return 8 * dk + static_cast<int>(chunk_of(r)) < blocks; };
-#pragma unroll
-    for (int j = 0; j < LA; ++j) {
-      const bool in = a_off[j] != kOOB && chunk_in(tile_row(j));
-      dma16(ra, in ? a_off[j] + ahead : kOOB, __builtin_amdgcn_readfirstlane(at + 1024 * (wave * LA + j)));
+  // DMA n of the cursor's stage into the ring stage at `at` (an offset out of range stays so).
+  auto fire = [&](int n, uint32_t at) __attribute__((always_inline)) {
+    const bool whole = 8 * dk + 8 <= blocks;
+    auto off = [&](uint32_t o, int chunk) { return whole || 8 * dk + chunk < blocks ? o + 128u * dk : kOOB; };
+    auto to = [&](int b) { return __builtin_amdgcn_readfirstlane(at + b); };
+    if (n < LB) {
+      dma16(rb, off(b_off[n], b_chunk(n)), to(kB + 1024 * (wave * LB + n)));
+    } else {
+      dma16(ra, off(a_off[n - LB], a_chunk(n - LB)), to(1024 * (wave * LA + n - LB)));
     }
-#pragma unroll
-    for (int j = 0; j < LB; ++j) {
-      const bool in = b_off[j] != kOOB && chunk_in(8 * (wave * LB + j) + l8);
-      dma16(rb, in ? b_off[j] + ahead : kOOB, __builtin_amdgcn_readfirstlane(at + kB + 1024 * (wave * LB + j)));
-    }
-    dma4(ras, as_off != kOOB ? as_off + 8u * dk : kOOB,
-         __builtin_amdgcn_readfirstlane(at + (32 * wave < BM ? kAs + 256 * wave : kSpare)));
-    dma4(rbs, bs_off != kOOB ? bs_off + 8u * dk : kOOB, __builtin_amdgcn_readfirstlane(at + kBs + 256 * wave));
+  };
+  int scales_to = 0, scales_at = 0;  // the scale ring's slots of the DMA and of the compute cursor
+  auto fire_scales = [&]() __attribute__((always_inline)) {  // with the first of two stages
+    if (dk & 1) return;
+    if (wave < kScaleWaves)
+      dma16(rs, s_off + 8u * dk, __builtin_amdgcn_readfirstlane(lds0 + STAGES * kStage + scales_to * kScales + 1024 * wave));
+    scales_to = scales_to + 1 == STAGES ? 0 : scales_to + 1;
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
     if (++dk == nk) seek();
   };
 
   // -------------------------------------------------------- compute cursor
-  const int a_lane = i16 * 128, swz = (i16 >> 1) & 7;
+  const int swz = i16 >> 1;  // a_key and b_key of the lane's fragment rows
+  const int a_lane = i16 * 128, b_row = 64 * wn + 16 * (i16 >> 2) + (i16 & 3);  // fragment j: rows b_row + 4 j
   f32x4_t acc[MT][NT];
-  auto multiply = [&](const char* st, int k, int rows) __attribute__((always_inline)) {
+  // acc += the stage at `st`, firing the DMA into the one at `to` on the way.
+  auto multiply = [&](const char* st, int k, int rows, uint32_t to) __attribute__((always_inline)) {
+    const char* sc = ring + STAGES * kStage + scales_at * kScales + (k & 1) * 8 + 2 * q;
     const int left = blocks - (8 * k + 2 * q);  // the lane's blocks inside K (scale padding may hold anything)
     const uint32_t keep = left > 1 ? 0xffffu : left > 0 ? 0xffu : 0u;
     uint32_t sw[NT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-      sw[j] = *reinterpret_cast<const uint16_t*>(st + kBs + (64 * wn + 16 * j + i16) * 8 + 2 * q) & keep;
+    for (int j = 0; j < NT; ++j) 
+      sw[j] = *reinterpret_cast<const uint16_t*>(sc + kBs + (64 * wn + 16 * j + i16) * 16) & keep;
     uint4 w[2][NT];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        w[s][j] = *reinterpret_cast<const uint4*>(st + kB + (64 * wn + 16 * j) * 128 + a_lane + (((2 * q + s) ^ swz) << 4));
+        w[s][j] = *reinterpret_cast<const uint4*>(st + kB + (b_row + 4 * j) * 128 + (((4 * s + q) ^ swz) << 4));
     // The next 16 rows' fragments are read while these are multiplied; tiles
     // without rows skip their products.
     uint4 a[2][2];
     uint32_t sa[2];
     auto read = [&](int i) __attribute__((always_inline)) {
       const int r = 16 * (wm + WM * i);
-      sa[i & 1] = *reinterpret_cast<const uint16_t*>(st + kAs + (r + i16) * 8 + 2 * q) & keep;
+      sa[i & 1] = *reinterpret_cast<const uint16_t*>(sc + (r + i16) * 16) & keep;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
-        a[i & 1][s] = *reinterpret_cast<const uint4*>(st + r * 128 + a_lane + (((2 * q + s) ^ swz) << 4));
+        a[i & 1][s] = *reinterpret_cast<const uint4*>(st + r * 128 + a_lane + (((4 * s + q) ^ swz) << 4));
     };
     read(0);
 #pragma unroll
@@ -231,87 +237,81 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = mx4_mfma<1>(w[1][j], a[i & 1][1], acc[i][j], sw[j], sa[i & 1]);
       }
+      if (i == 0) fire_scales();
+#pragma unroll
+      for (int n = i * LPW / kFire; i < kFire && n < (i + 1) * LPW / kFire; ++n) fire(n, to);
     }
+    advance();
+    if ((k & 1) || k + 1 == nk) scales_at = scales_at + 1 == STAGES ? 0 : scales_at + 1;
   };
-  auto store = [&](char* st, const Mx4Tile& t) __attribute__((always_inline)) {
-    char* mine = st + wave * kSlot;
-    const int n0 = t.n * kCols + wn * (kCols / 4);  // the wave's first output column
-    if constexpr (EPI == MX4_SWIGLU_MX4) {
-      const auto rc = make_rsrc(p.c_codes + static_cast<int64_t>(t.r0) * (p.N / 2), static_cast<uint32_t>(t.rows) * (p.N / 2));
-      const uint32_t out_pitch = static_cast<uint32_t>(mx4_pitch(p.N));
-      const auto rs = make_rsrc(p.c_scales + static_cast<int64_t>(t.r0) * out_pitch, static_cast<uint32_t>(t.rows) * out_pitch);
+  // The tile's results: lane l holds row 16 (wm + 2 i) + l % 16, and of the wave's columns 16 q + 4 j .. + 3 in
+  // acc[i][j], or gate and up of act columns 8 q + 4 h .. + 3 in acc[i][2 h] and [2 h + 1].
+  auto store = [&](const Mx4Tile& t) __attribute__((always_inline)) {
+    auto put16 = [](__amdgpu_buffer_rsrc_t rs, uint32_t off, const float (&o)[8]) {
+      __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
+                                                     pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])}, rs, off, 0, 0);
+    };
+    const uint32_t N = p.N;
+    const uint32_t n0 = t.n * kCols + wn * (kCols / 4);  // the wave's first output column
+    const auto rc = make_rsrc(p.c + static_cast<int64_t>(t.r0) * N, static_cast<uint32_t>(t.rows) * N * 2u);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        float act[2][4];
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          act[e / 4][e % 4] = silu_f(acc[i][2 * (e / 4)][e % 4]) * acc[i][2 * (e / 4) + 1][e % 4];
-          top = max(top, __float_as_uint(act[e / 4][e % 4]) & 0x7fffffffu);
-        }
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-        const uint32_t s = mx4_scale(top);
-        const float f = mx4_scale_f(s);
+    for (int i = 0; i < MT; ++i) {
+      const uint32_t row = 16 * (wm + WM * i) + i16;
+      const bool in = static_cast<int>(row) < t.rows;
+      if constexpr (EPI == MX4_PLAIN) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          const uint32_t n = n0 + 16 * q + 8 * h;
+          float o[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = acc[i][2 * h + e / 4][e % 4];
+          put16(rc, in && n < N ? (row * N + n) * 2u : kOOB, o);
+        }
+      } else {
+        float act[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) act[e] = mx4_act(acc[i][2 * (e / 4)][e % 4], acc[i][2 * (e / 4) + 1][e % 4]);
+        if constexpr (EPI == MX4_SWIGLU) {
+          const uint32_t n = n0 + 8 * q;
+          put16(rc, in && n < N ? (row * N + n) * 2u : kOOB, act);
+        } else {  // quantised from fp32: one rounding, to 4 bits
+          const uint32_t out_pitch = static_cast<uint32_t>(mx4_pitch(N));
+          const auto rcc = make_rsrc(p.c_codes + static_cast<int64_t>(t.r0) * (N / 2), static_cast<uint32_t>(t.rows) * (N / 2));
+          const auto rcs = make_rsrc(p.c_scales + static_cast<int64_t>(t.r0) * out_pitch,
+                                     static_cast<uint32_t>(t.rows) * out_pitch);
+          uint32_t top = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(act[e]) & 0x7fffffffu);
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
+          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+          const uint32_t s = mx4_scale(top);
+          const float f = mx4_scale_f(s);
           uint32_t c = 0;
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[h][0], act[h][1], f, 0);
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[h][2], act[h][3], f, 1);
-          *reinterpret_cast<uint16_t*>(mine + (16 * i + i16) * 16 + 8 * h + 2 * q) =
-              static_cast<uint16_t>(s == 255u ? 0u : c);
-        }
-        if (q == 0) mine[MT * 256 + 16 * i + i16] = static_cast<char>(s);
-      }
-#pragma unroll
-      for (int h = 0; h < (MT * 16 + 63) / 64; ++h) {
-        const int m = 64 * h + lane;                              // of the wave's rows
-        const int row = 16 * (wm + WM * (m >> 4)) + (m & 15);     // of the tile's
-        const bool in = m < MT * 16 && row < t.rows && n0 < p.N;
-        const uint4 v = *reinterpret_cast<const uint4*>(mine + (m < MT * 16 ? m : 0) * 16);
-        const uint8_t s = static_cast<uint8_t>(mine[MT * 256 + (m < MT * 16 ? m : 0)]);
-        __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{v.x, v.y, v.z, v.w}, rc,
-                                               in ? static_cast<uint32_t>(row) * (p.N / 2) + n0 / 2 : kOOB, 0, 0);
-        __builtin_amdgcn_raw_buffer_store_b8(s, rs, in ? static_cast<uint32_t>(row) * out_pitch + n0 / 32 : kOOB, 0, 0);
-      }
-    } else {
-      constexpr int W = GLU ? 32 : 64;         // the wave's output columns
-      constexpr int kRow = 2 * W + 16;         // staged row: neighbouring rows on other banks
-      constexpr int kPieces = W / 8, kPass = 64 / kPieces;
-      const auto rc = make_rsrc(p.c + static_cast<int64_t>(t.r0) * p.N, static_cast<uint32_t>(t.rows) * p.N * 2u);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-#pragma unroll
-        for (int j = 0; j < W / 16; ++j) {
-          float o[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (GLU) o[e] = silu_f(acc[i][2 * j][e]) * acc[i][2 * j + 1][e];
-            else o[e] = acc[i][j][e];
-          }
-          *reinterpret_cast<uint2*>(mine + i16 * kRow + (16 * j + 4 * q) * 2) =
-              make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
-        }
-#pragma unroll
-        for (int h = 0; h < 16 / kPass; ++h) {
-          const int r = h * kPass + lane / kPieces, piece = lane % kPieces;
-          const uint4 v = *reinterpret_cast<const uint4*>(mine + r * kRow + 16 * piece);
-          const int row = 16 * (wm + WM * i) + r, n = n0 + 8 * piece;
-          const bool in = row < t.rows && n < p.N;
-          __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{v.x, v.y, v.z, v.w}, rc,
-                                                 in ? (static_cast<uint32_t>(row) * p.N + n) * 2u : kOOB, 0, 0);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[0], act[1], f, 0);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[2], act[3], f, 1);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[4], act[5], f, 2);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[6], act[7], f, 3);
+          const bool w = in && n0 < N;
+          __builtin_amdgcn_raw_buffer_store_b32(s == 255u ? 0u : c, rcc, w ? row * (N / 2) + n0 / 2 + 4 * q : kOOB, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(s), rcs, w && q == 0 ? row * out_pitch + n0 / 32 : kOOB,
+                                               0, 0);
         }
       }
     }
   };
 
+  hold(0);
   fetch_rows(0);
   seek();
+  for (int s = 0; s < STAGES - 1; ++s) {
+    fire_scales();
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) issue(s);
+    for (int n = 0; n < LPW; ++n) fire(n, lds0 + s * kStage);
+    advance();
+  }
   int at = 0, since = STAGES;  // the ring's stage, steps since an epilogue
-  for (int j = 0; j < ntiles; ++j) {
-    const Mx4Tile t = find(j);
+  for (; cj < ntiles; ++cj) {
+    const Mx4Tile t = find(cj);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -327,21 +327,12 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
       wait_lgkmcnt0();               // this wave's reads of the stage before are done
       __builtin_amdgcn_s_barrier();  // every wave's share landed, and all have left the stage the DMA turns to
       asm volatile("" ::: "memory");
-      issue(at ? at - 1 : STAGES - 1);
-      __builtin_amdgcn_s_setprio(1);
-      multiply(ring + at * kStage, k, t.rows);
-      __builtin_amdgcn_s_setprio(0);
+      multiply(ring + at * kStage, k, t.rows, lds0 + (at ? at - 1 : STAGES - 1) * kStage);
       ++since;
-      if (k + 1 < nk) at = at + 1 == STAGES ? 0 : at + 1;
+      at = at + 1 == STAGES ? 0 : at + 1;
     }
-    asm volatile("" ::: "memory");
-    wait_lgkmcnt0();
-    __builtin_amdgcn_s_barrier();  // all have read the stage that the epilogue writes through
-    asm volatile("" ::: "memory");
-    store(ring + at * kStage, t);
+    store(t);
     since = 0;
-    at = at + 1 == STAGES ? 0 : at + 1;
-    wait_lgkmcnt0();  // the staging is read before the next barrier lets the DMA into it
   }
   wait_vmcnt<0>();  // the trailing DMA (out of range: zeros) before the LDS is released
 }
@@ -368,7 +359,7 @@ int launch(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name) {
 
 int mx4_tile(const Mx4Gemm& p, int epi, int bm, hipStream_t stream, const char* name) {
   return bm <= 64 ? launch<64, 3>(p, epi, stream, name)
-                  : bm <= 128 ? launch<128, 3>(p, epi, stream, name) : launch<256, 2>(p, epi, stream, name);
+                  : bm <= 128 ? launch<128, 2>(p, epi, stream, name) : launch<256, 2>(p, epi, stream, name);
 }
 
 }  // namespace moe
