@@ -482,6 +482,22 @@ int moe_mx4_grouped_swiglu(const void* a_codes, const void* a_scales,
                            void* act, void* act_codes, void* act_scales,
                            void* stream);
 
+/* A layer's routed experts on mx4 weights, all launches of it: the slots
+ * T x k sorted by ids (ids outside [0, E) contribute nothing), hidden [T, H]
+ * (bf16, or f32 with is_f32) quantised, gate_up [E, 2I, H] with the SwiGLU
+ * output quantised, down [E, H, I], and out [T, H] (hidden's type) = the
+ * weights' [T, k] (f32) sum of each token's rows in fp32.  Rows of down are
+ * f32 for f32 hidden states and up to 4M values, else bf16.  H and I are
+ * multiples of 32, k at most 16, E at most 1024. */
+size_t moe_mx4_experts_workspace_bytes(int is_f32, int64_t T, int64_t H,
+                                       int64_t k, int64_t E, int64_t I);
+int moe_mx4_experts(const void* hidden, int is_f32, const int64_t* ids,
+                    const float* weights, int64_t T, int64_t H, int64_t k,
+                    int64_t E, int64_t I, const void* gate_up_codes,
+                    const void* gate_up_scales, const void* down_codes,
+                    const void* down_scales, void* out, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------ the fp32 expert path */
 
 /* The reference's grouped experts accept fp32 modules and then compute in

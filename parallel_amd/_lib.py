@@ -84,6 +84,8 @@ SIGNATURES: dict[str, tuple] = {
     "moe_mx4_dequantize": (_I, [_P, _P, _I64, _I64, _I, _P, _P]),
     "moe_mx4_grouped_gemm": (_I, [_P, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P]),
     "moe_mx4_grouped_swiglu": (_I, [_P, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _P, _P]),
+    "moe_mx4_experts_workspace_bytes": (_SZ, [_I, _I64, _I64, _I64, _I64, _I64]),
+    "moe_mx4_experts": (_I, [_P, _I, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "moe_router_aux_fwd_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
     "moe_router_aux_fwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _SZ, _P]),
 }

@@ -42,9 +42,11 @@ struct Mx4Gemm {
   const int32_t* offs;
   int G, rows, N, K;
   bf16_t* c;                    // [rows, N] bf16, or
-  uint8_t *c_codes, *c_scales;  // (swiglu only) [rows, N] as mx4
+  float* c32;                   // (without swiglu) f32, or
+  uint8_t *c_codes, *c_scales;  // (with swiglu) mx4
 };
-enum { MX4_PLAIN = 0, MX4_SWIGLU = 1, MX4_SWIGLU_MX4 = 2 };
+enum { MX4_PLAIN = 0, MX4_SWIGLU = 1, MX4_SWIGLU_MX4 = 2, MX4_PLAIN_F32 = 3 };
+constexpr bool mx4_glu(int epi) { return epi == MX4_SWIGLU || epi == MX4_SWIGLU_MX4; }
 
 // Rows of group g, clamped so that malformed offsets never address outside [0, rows).
 __device__ __forceinline__ int mx4_group_rows(const Mx4Gemm& p, int g, int& lo) {
@@ -130,63 +132,10 @@ __device__ __forceinline__ f32x4_t mx4_mfma(const uint4& w, const uint4& a, cons
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, af, c, 4, 4, STEP, sw, STEP, sa);
 }
 
-// A 16-row result with four column tiles per lane (v[j]: columns 16 j + 4 q ..
-// of row `row`, q = lane / 16; with swiglu the tiles alternate gate and up)
-// written to columns n0 .. of the output.
-template <int EPI, int NT>
-__device__ __forceinline__ void mx4_store_rows(const Mx4Gemm& p, const f32x4_t (&v)[NT], int64_t row, bool in, int n0,
-                                               int q) {
-  if constexpr (EPI == MX4_PLAIN) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int n = n0 + 16 * j + 4 * q;
-      if (in && n < p.N)
-        *reinterpret_cast<uint2*>(p.c + row * p.N + n) =
-            make_uint2(pack_bf16x2(v[j][0], v[j][1]), pack_bf16x2(v[j][2], v[j][3]));
-    }
-  } else {
-    float act[NT / 2][4];
-#pragma unroll
-    for (int j = 0; j < NT / 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) act[j][e] = mx4_act(v[2 * j][e], v[2 * j + 1][e]);
-    if constexpr (EPI == MX4_SWIGLU) {
-#pragma unroll
-      for (int j = 0; j < NT / 2; ++j) {
-        const int n = n0 + 16 * j + 4 * q;
-        if (in && n < p.N)
-          *reinterpret_cast<uint2*>(p.c + row * p.N + n) =
-              make_uint2(pack_bf16x2(act[j][0], act[j][1]), pack_bf16x2(act[j][2], act[j][3]));
-      }
-    } else {
-      static_assert(NT % 4 == 0, "a 32-value block is two act tiles");
-#pragma unroll
-      for (int j = 0; j < NT / 2; j += 2) {  // quantised from fp32: one rounding, to 4 bits
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(act[j + e / 4][e % 4]) & 0x7fffffffu);
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-        top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
-        const uint32_t s = mx4_scale(top);
-        const float f = mx4_scale_f(s);
-        const int n = n0 + 16 * j;
-        if (!in || n >= p.N) continue;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t c = 0;
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[j + h][0], act[j + h][1], f, 0);
-          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[j + h][2], act[j + h][3], f, 1);
-          if (s == 255u) c = 0;
-          *reinterpret_cast<uint16_t*>(p.c_codes + row * (p.N / 2) + (n + 16 * h + 4 * q) / 2) =
-              static_cast<uint16_t>(c);
-        }
-        if (q == 0) p.c_scales[row * mx4_pitch(p.N) + n / 32] = static_cast<uint8_t>(s);
-      }
-    }
-  }
-}
+// Blocks of the few-row kernel side by side over N output columns.
+inline int64_t mx4_few_columns(int64_t N, int epi) { return mx4_glu(epi) ? (N + 31) / 32 : (N + 63) / 64; }
 
-// Products of few rows per group (mx4_few.hip).
+// Products of few tiles in all (mx4_few.hip).
 int mx4_few(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name);
 // Products of many rows per group in tiles of up to bm (64, 128 or 256) rows (mx4_tile.hip).
 int mx4_tile(const Mx4Gemm& p, int epi, int bm, hipStream_t stream, const char* name);

@@ -94,6 +94,38 @@ __global__ __launch_bounds__(kMx4Threads) void mx4_dequantize_kernel(const uint3
   }
 }
 
+// out[t, :] = sum over the token's slots, in slot order, of weight * row (fp32 rows), 8 columns a thread.
+template <class E>
+__global__ __launch_bounds__(kMx4Threads) void mx4_combine_kernel(const float* __restrict__ y,
+                                                                  const int32_t* __restrict__ pos_of_slot,
+                                                                  const int32_t* __restrict__ offsets, int E_,
+                                                                  const float* __restrict__ weights, int H, int k,
+                                                                  int per_row, E* __restrict__ out) {
+  const int64_t t = blockIdx.x / per_row;
+  const int c = (blockIdx.x % per_row) * kMx4Threads + threadIdx.x;
+  if (c >= H / 8) return;
+  const int valid = offsets[E_ - 1];
+  float o[8] = {};
+#pragma unroll 4
+  for (int j = 0; j < k; ++j) {
+    const int pos = pos_of_slot[t * k + j];
+    if (pos >= valid) continue;  // the slot's expert is elsewhere
+    const float w = weights[t * k + j];
+    const float4* row = reinterpret_cast<const float4*>(y + static_cast<int64_t>(pos) * H + 8 * c);
+    const float4 a = row[0], b = row[1];
+    o[0] += w * a.x; o[1] += w * a.y; o[2] += w * a.z; o[3] += w * a.w;
+    o[4] += w * b.x; o[5] += w * b.y; o[6] += w * b.z; o[7] += w * b.w;
+  }
+  if constexpr (std::is_same<E, float>::value) {
+    float4* to = reinterpret_cast<float4*>(out + t * H + 8 * c);
+    to[0] = make_float4(o[0], o[1], o[2], o[3]);
+    to[1] = make_float4(o[4], o[5], o[6], o[7]);
+  } else {
+    *reinterpret_cast<uint4*>(out + t * H + 8 * c) = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
+                                                                pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+  }
+}
+
 }  // namespace moe
 
 using namespace moe;
@@ -119,16 +151,31 @@ unsigned pass_blocks(int64_t n8) {
   return static_cast<unsigned>(blocks < 16384 ? blocks : 16384);
 }
 
+// Which kernel, from the rows and groups alone (the groups' own counts are on the device).
+// The few-row kernel where it needs at most 512 blocks (16 rows by 64 weight rows each) and groups are small: it
+// is then ahead of 64-row tiles or level (mx4_few.hip has the times).  Tiles of 64, 128 or 256 rows by the mean:
+// gate and up of 128 groups, 2048 x 768, at 32, 64, 96, 128, 256 and 1024 rows each take
+//   64-row tiles 37, 47, 55, 72, 129, 433 us; 128-row 42, 44, 47, 63, 120, 360; 256-row 51, 52, 55, 58, 107, 292,
+// the down products of 64 Zipf groups with 156 rows in the mean 30 us with 128 rows and 39 with 256, a uniform
+// 160 12% less with 256: routing is skewed more often than not.
+int mx4_product(const Mx4Gemm& p, int epi, hipStream_t stream, const char* what) {
+  const int64_t mean = (static_cast<int64_t>(p.rows) + p.G - 1) / p.G;
+  const int64_t groups = p.G < p.rows ? p.G : p.rows;
+  if (mean <= 64 && (groups + (p.rows - groups) / 16) * mx4_few_columns(p.N, epi) <= 512)
+    return mx4_few(p, epi, stream, what);
+  return mx4_tile(p, epi, mean <= 56 ? 64 : mean <= 160 ? 128 : 256, stream, what);
+}
+
 int run_product(const char* what, const void* a, const void* a_scales, int64_t a_rows, const int32_t* row_index,
                 int64_t row_div, const void* w, const void* w_scales, const int32_t* offs, int64_t G, int64_t M,
                 int64_t N, int64_t K, void* c, void* c_codes, void* c_scales, int epi, void* stream) {
-  const int64_t wide = epi == MX4_PLAIN ? N : 2 * N;
+  const int64_t wide = mx4_glu(epi) ? 2 * N : N;
   MOE_REQUIRE(G > 0 && M >= 0 && a_rows >= 0 && N > 0 && K > 0 && row_div > 0, MOE_ERR_INVALID, "%s: bad sizes", what);
   MOE_REQUIRE(K % 32 == 0 && N % 8 == 0, MOE_ERR_UNSUPPORTED, "%s: K=%lld must be a multiple of 32, N=%lld of 8", what,
               (long long)K, (long long)N);
   MOE_REQUIRE(epi != MX4_SWIGLU_MX4 || N % 32 == 0, MOE_ERR_UNSUPPORTED,
               "%s: 4-bit output of %lld columns is not whole blocks of 32", what, (long long)N);
-  MOE_REQUIRE(M < (1ll << 31) && a_rows < (1ll << 31) && G < (1ll << 24) && row_div < (1ll << 31) && N < (1ll << 28) &&
+  MOE_REQUIRE(M < (1ll << 31) && a_rows < (1ll << 31) && G < (1ll << 24) && row_div < (1ll << 31) && N <= (1ll << 20) &&
                   K < (1ll << 28),
               MOE_ERR_UNSUPPORTED, "%s: sizes past 32 bits", what);
   MOE_REQUIRE(a_rows * (K / 2) < (1ll << 31) && wide * (K / 2) < (1ll << 31), MOE_ERR_UNSUPPORTED,
@@ -163,12 +210,11 @@ int run_product(const char* what, const void* a, const void* a_scales, int64_t a
   p.rows = static_cast<int>(M);
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
-  p.c = static_cast<bf16_t*>(c);
+  if (epi == MX4_PLAIN_F32) p.c32 = static_cast<float*>(c);
+  else p.c = static_cast<bf16_t*>(c);
   p.c_codes = static_cast<uint8_t*>(c_codes);
   p.c_scales = static_cast<uint8_t*>(c_scales);
-  const int64_t mean = (M + G - 1) / G;
-  if (mean <= 32) return mx4_few(p, epi, as_stream(stream), what);
-  return mx4_tile(p, epi, mean <= 64 ? 64 : mean <= 128 ? 128 : 256, as_stream(stream), what);
+  return mx4_product(p, epi, as_stream(stream), what);
 }
 }  // namespace
 
@@ -220,4 +266,92 @@ extern "C" int moe_mx4_grouped_swiglu(const void* a_codes, const void* a_scales,
                                       int64_t K, void* act, void* act_codes, void* act_scales, void* stream) {
   return run_product("moe_mx4_grouped_swiglu", a_codes, a_scales, a_rows, row_index, row_divisor, w_codes, w_scales,
                      offs, G, M, I, K, act, act_codes, act_scales, act_codes ? MX4_SWIGLU_MX4 : MX4_SWIGLU, stream);
+}
+
+namespace {
+// The experts' workspace, each part 256-byte aligned.
+struct ExpertsSpace {
+  size_t perm, pos, counts, offsets, sort, x, x_scales, act, act_scales, y, bytes;
+  size_t sort_bytes;
+  bool f32_rows;
+};
+// The down product's rows are held in fp32 for fp32 modules, and while they stay small enough (16 MiB) that their
+// bytes do not count; a bf16 row rounds once more, by half a step of the output's type.
+ExpertsSpace experts_space(bool is_f32, int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
+  const int64_t S = T * k;
+  ExpertsSpace s{};
+  size_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const size_t here = at;
+    at += (static_cast<size_t>(bytes) + 255) / 256 * 256;
+    return here;
+  };
+  s.f32_rows = is_f32 || S * H <= (1ll << 22);
+  s.perm = take(4 * S);
+  s.pos = take(4 * S);
+  s.counts = take(4 * E);
+  s.offsets = take(4 * E);
+  s.sort_bytes = moe_permute_workspace_bytes(S, E);
+  s.sort = take(static_cast<int64_t>(s.sort_bytes));
+  s.x = take(T * (H / 2));
+  s.x_scales = take(T * mx4_pitch(H));
+  s.act = take(S * (I / 2));
+  s.act_scales = take(S * mx4_pitch(I));
+  s.y = take(S * H * (s.f32_rows ? 4 : 2));
+  s.bytes = at;
+  return s;
+}
+bool experts_sizes(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
+  return T >= 0 && T < (1ll << 31) && k >= 1 && k <= kMaxSlots && T * k < (1ll << 31) && E >= 1 && H > 0 &&
+         H <= (1ll << 20) && I > 0 && I <= (1ll << 20);
+}
+}  // namespace
+
+extern "C" size_t moe_mx4_experts_workspace_bytes(int is_f32, int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
+  return experts_sizes(T, H, k, E, I) ? experts_space(is_f32, T, H, k, E, I).bytes : 0;
+}
+
+extern "C" int moe_mx4_experts(const void* hidden, int is_f32, const int64_t* ids, const float* weights, int64_t T,
+                               int64_t H, int64_t k, int64_t E, int64_t I, const void* gate_up_codes,
+                               const void* gate_up_scales, const void* down_codes, const void* down_scales, void* out,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  MOE_REQUIRE(experts_sizes(T, H, k, E, I), MOE_ERR_INVALID, "mx4 experts: bad sizes (k at most %d)", kMaxSlots);
+  MOE_REQUIRE(H % 32 == 0 && I % 32 == 0, MOE_ERR_UNSUPPORTED, "mx4 experts: H=%lld and I=%lld must be multiples of 32",
+              (long long)H, (long long)I);
+  if (T == 0) return MOE_OK;
+  MOE_REQUIRE(hidden && ids && weights && out && aligned16(hidden) && aligned16(out), MOE_ERR_INVALID,
+              "mx4 experts: bad pointer");
+  const ExpertsSpace s = experts_space(is_f32, T, H, k, E, I);
+  MOE_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= s.bytes, MOE_ERR_WORKSPACE,
+              "mx4 experts: workspace %zu < %zu bytes", workspace_bytes, s.bytes);
+  char* ws = static_cast<char*>(workspace);
+  int32_t* perm = reinterpret_cast<int32_t*>(ws + s.perm);
+  int32_t* pos = reinterpret_cast<int32_t*>(ws + s.pos);
+  int32_t* offsets = reinterpret_cast<int32_t*>(ws + s.offsets);
+  const int64_t S = T * k;
+  int rc = permute_fwd_run(nullptr, T, 0, ids, k, 1, E, nullptr, perm, pos, reinterpret_cast<int32_t*>(ws + s.counts),
+                           offsets, ws + s.sort, s.sort_bytes, stream);
+  if (rc) return rc;
+  rc = moe_mx4_quantize(hidden, is_f32, T, H, ws + s.x, ws + s.x_scales, stream);
+  if (rc) return rc;
+  rc = run_product("mx4 experts, gate and up", ws + s.x, ws + s.x_scales, T, perm, k, gate_up_codes, gate_up_scales,
+                   offsets, E, S, I, H, nullptr, ws + s.act, ws + s.act_scales, MX4_SWIGLU_MX4, stream);
+  if (rc) return rc;
+  rc = run_product("mx4 experts, down", ws + s.act, ws + s.act_scales, S, nullptr, 1, down_codes, down_scales, offsets,
+                   E, S, H, I, ws + s.y, nullptr, nullptr, s.f32_rows ? MX4_PLAIN_F32 : MX4_PLAIN, stream);
+  if (rc) return rc;
+  if (!s.f32_rows) return moe_combine_fwd(ws + s.y, pos, offsets, E, weights, T, H, k, out, stream);
+  const int64_t per_row = (H / 8 + kMx4Threads - 1) / kMx4Threads;
+  MOE_REQUIRE(T * per_row < (1ll << 31), MOE_ERR_UNSUPPORTED, "mx4 experts: too many rows");
+  const dim3 grid(static_cast<unsigned>(T * per_row)), block(kMx4Threads);
+  const float* y = reinterpret_cast<const float*>(ws + s.y);
+  if (is_f32)
+    hipLaunchKernelGGL(mx4_combine_kernel<float>, grid, block, 0, as_stream(stream), y, pos, offsets,
+                       static_cast<int>(E), weights, static_cast<int>(H), static_cast<int>(k),
+                       static_cast<int>(per_row), static_cast<float*>(out));
+  else
+    hipLaunchKernelGGL(mx4_combine_kernel<bf16_t>, grid, block, 0, as_stream(stream), y, pos, offsets,
+                       static_cast<int>(E), weights, static_cast<int>(H), static_cast<int>(k),
+                       static_cast<int>(per_row), static_cast<bf16_t*>(out));
+  return launch_status("moe_mx4_experts(combine)");
 }

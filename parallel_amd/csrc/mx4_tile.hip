@@ -10,8 +10,8 @@
 // two scales one 16-bit read.  The scales come 16 bytes (two stages) of a row
 // at a time into a ring of their own: fetched stage by stage they were as many
 // L2 requests as the codes' whole lines.  The wave's 64 weight rows are dealt to its four
-// fragments four rows at a time, so that a lane's results are 16 neighbouring
-// output columns of one row (8 act columns with swiglu), stored as they are.
+// fragments four rows at a time, so that a lane's results are twice 8 (with
+// swiglu once) neighbouring output columns of one row, stored as they are.
 //
 // Blocks are persistent, one per CU, and run one stream of stages over their
 // tiles: a DMA cursor (buffer_load ... lds, fired between the products) fills a
@@ -42,7 +42,7 @@ __device__ __forceinline__ void each_groups(const Mx4Gemm& p, F&& f) {
 
 template <int BM, int STAGES, int EPI>
 __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p, int n_tiles) {
-  constexpr bool GLU = EPI != MX4_PLAIN;
+  constexpr bool GLU = mx4_glu(EPI);
   constexpr int WM = 2, MT = BM / 16 / WM, NT = 4;
   constexpr int kCols = GLU ? kTileN / 2 : kTileN;     // output columns per tile
   constexpr int LA = BM / 64, LB = kTileN / 64;        // code DMAs per wave and stage (8 rows each)
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
   constexpr int kB = BM * 128, kStage = kB + kTileN * 128;
   constexpr int kScaleWaves = (BM + kTileN) / 64;      // waves that fetch scales, 64 rows each: A's, then B's
   constexpr int kScales = kScaleWaves * 1024, kBs = BM * 16;
-  constexpr int kStores = EPI == MX4_SWIGLU ? MT : 2 * MT;  // store instructions per wave and tile
+  constexpr int kStores = EPI == MX4_SWIGLU ? MT : EPI == MX4_PLAIN_F32 ? 4 * MT : 2 * MT;  // store instructions per wave and tile
   // 16-row tiles between whose products the next stage's DMA is fired: a ring of two needs it early.
   constexpr int kFire = STAGES == 2 ? MT / 2 : MT;
   static_assert(kScaleWaves <= kTileWaves && STAGES * (kStage + kScales) <= 160 * 1024, "LDS");
@@ -159,7 +159,8 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
     for (int j = 0; j < LA; ++j) a_off[j] = source(j, half_k, 16u * a_chunk(j));
     auto weight = [&](int r, uint32_t row_bytes, uint32_t off) {  // row r of the tile's: fragment (r / 4) % 4
       const int j = (r >> 2) & 3;
-      const int n = t.n * kCols + (GLU ? (r >> 6) * 32 + ((r >> 4) & 3) * 8 + (j >> 1) * 4 + (r & 3) : r);
+      const int n = t.n * kCols + (GLU ? (r >> 6) * 32 + ((r >> 4) & 3) * 8 + (j >> 1) * 4 + (r & 3)
+                                      : (r & ~63) + (j >> 1) * 32 + ((r >> 4) & 3) * 8 + (j & 1) * 4 + (r & 3));
       const int w = GLU && (j & 1) ? p.N + n : n;
       return live && n < p.N ? static_cast<uint32_t>(w) * row_bytes + off : kOOB;
     };
@@ -244,8 +245,8 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
     advance();
     if ((k & 1) || k + 1 == nk) scales_at = scales_at + 1 == STAGES ? 0 : scales_at + 1;
   };
-  // The tile's results: lane l holds row 16 (wm + 2 i) + l % 16, and of the wave's columns 16 q + 4 j .. + 3 in
-  // acc[i][j], or gate and up of act columns 8 q + 4 h .. + 3 in acc[i][2 h] and [2 h + 1].
+  // The tile's results: lane l holds row 16 (wm + 2 i) + l % 16, and of the wave's columns 32 (j / 2) + 8 q + 4 (j %
+  // 2) .. + 3 in acc[i][j], or gate and up of act columns 8 q + 4 h .. + 3 in acc[i][2 h] and [2 h + 1].
   auto store = [&](const Mx4Tile& t) __attribute__((always_inline)) {
     auto put16 = [](__amdgpu_buffer_rsrc_t rs, uint32_t off, const float (&o)[8]) {
       __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
@@ -253,15 +254,24 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
     };
     const uint32_t N = p.N;
     const uint32_t n0 = t.n * kCols + wn * (kCols / 4);  // the wave's first output column
-    const auto rc = make_rsrc(p.c + static_cast<int64_t>(t.r0) * N, static_cast<uint32_t>(t.rows) * N * 2u);
+    const auto rc = EPI == MX4_PLAIN_F32
+                        ? make_rsrc(p.c32 + static_cast<int64_t>(t.r0) * N, static_cast<uint32_t>(t.rows) * N * 4u)
+                        : make_rsrc(p.c + static_cast<int64_t>(t.r0) * N, static_cast<uint32_t>(t.rows) * N * 2u);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const uint32_t row = 16 * (wm + WM * i) + i16;
       const bool in = static_cast<int>(row) < t.rows;
-      if constexpr (EPI == MX4_PLAIN) {
+      if constexpr (EPI == MX4_PLAIN_F32) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const uint32_t n = n0 + 32 * (j / 2) + 8 * q + 4 * (j % 2);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[i][j]), rc,
+                                                 in && n < N ? (row * N + n) * 4u : kOOB, 0, 0);
+        }
+      } else if constexpr (EPI == MX4_PLAIN) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t n = n0 + 16 * q + 8 * h;
+          const uint32_t n = n0 + 32 * h + 8 * q;
           float o[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = acc[i][2 * h + e / 4][e % 4];
@@ -339,7 +349,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
 
 template <int BM, int STAGES>
 int launch(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name) {
-  const int cols = epi == MX4_PLAIN ? kTileN : kTileN / 2;
+  const int cols = mx4_glu(epi) ? kTileN / 2 : kTileN;
   const int n_tiles = (p.N + cols - 1) / cols;
   const int64_t most = mx4_most_tiles(p.rows, p.G, BM) * n_tiles;
   MOE_REQUIRE(most < (1ll << 30), MOE_ERR_UNSUPPORTED, "%s: too many tiles", name);
@@ -348,6 +358,8 @@ int launch(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name) {
   const dim3 grid(static_cast<unsigned>(want < cus ? want : cus)), block(kTileThreads);
   if (epi == MX4_PLAIN)
     hipLaunchKernelGGL((mx4_tile_kernel<BM, STAGES, MX4_PLAIN>), grid, block, 0, stream, p, n_tiles);
+  else if (epi == MX4_PLAIN_F32)
+    hipLaunchKernelGGL((mx4_tile_kernel<BM, STAGES, MX4_PLAIN_F32>), grid, block, 0, stream, p, n_tiles);
   else if (epi == MX4_SWIGLU)
     hipLaunchKernelGGL((mx4_tile_kernel<BM, STAGES, MX4_SWIGLU>), grid, block, 0, stream, p, n_tiles);
   else

@@ -919,36 +919,22 @@ def _check_mx4_experts(hidden, top_k_index, top_k_weights, gu_codes, gu_scales, 
 @_op("mx4_experts")
 def mx4_experts(hidden: Tensor, top_k_index: Tensor, top_k_weights: Tensor, gate_up_codes: Tensor,
                 gate_up_scales: Tensor, down_codes: Tensor, down_scales: Tensor) -> Tensor:
-    """experts_fwd on 4-bit weights: the tokens are quantised once, the sorted slots read them through the sort's
-    order, the act values are quantised as they are formed, and the combine sums bf16 rows in fp32."""
+    """experts_fwd on 4-bit weights, [T, H] like hidden: the tokens are quantised once, the sorted slots read them
+    through the sort's order, the act values are quantised as they are formed, and the combine sums in fp32."""
     T, H, k, E, I = _check_mx4_experts(hidden, top_k_index, top_k_weights, gate_up_codes, gate_up_scales, down_codes,
                                        down_scales)
-    S = T * k
-    dev = hidden.device
-    out = torch.empty(T, H, dtype=BF16, device=dev)
-    if S == 0:
-        return out.zero_().to(hidden.dtype)
-    ids, w = _ids64(top_k_index), top_k_weights.float().contiguous()
+    ids, w = _ids64(top_k_index), _rows16(top_k_weights.float())
     weights = tuple(map(_rows16, (gate_up_codes, gate_up_scales, down_codes, down_scales)))
-    u8 = dict(dtype=torch.uint8, device=dev)
+    f32 = int(hidden.dtype == torch.float32)
     x = _rows16(hidden)
+    out = torch.empty(T, H, dtype=hidden.dtype, device=hidden.device)
+    if k == 0:
+        return out.zero_()
     with _device(hidden):
-        s = _stream(hidden)
-        perm, pos = torch.empty(2, S, dtype=torch.int32, device=dev).unbind()
-        counts, offsets = torch.empty(2, E, dtype=torch.int32, device=dev).unbind()
-        ws = _ws(_lib.load().moe_permute_workspace_bytes(S, E), dev)
-        call("moe_permute_fwd", None, T, 0, ptr(ids), k, 1, E, None, ptr(perm), ptr(pos), ptr(counts), ptr(offsets),
-             ptr(ws), ws.numel(), s, tag="permute_fwd")
-        xc, xs = torch.empty(T, H // 2, **u8), torch.empty(T, mx4_pitch(H), **u8)
-        call("moe_mx4_quantize", ptr(x), int(x.dtype == torch.float32), T, H, ptr(xc), ptr(xs), s, tag="mx4_quantize")
-        ac, asc = torch.empty(S, I // 2, **u8), torch.empty(S, mx4_pitch(I), **u8)
-        call("moe_mx4_grouped_swiglu", ptr(xc), ptr(xs), T, ptr(perm), k, ptr(weights[0]), ptr(weights[1]),
-             ptr(offsets), E, S, I, H, None, ptr(ac), ptr(asc), s, tag="mx4_up")
-        y = torch.empty(S, H, dtype=BF16, device=dev)
-        call("moe_mx4_grouped_gemm", ptr(ac), ptr(asc), S, None, 1, ptr(weights[2]), ptr(weights[3]), ptr(offsets), E,
-             S, H, I, ptr(y), s, tag="mx4_down")
-        call("moe_combine_fwd", ptr(y), ptr(pos), ptr(offsets), E, ptr(w), T, H, k, ptr(out), s, tag="combine_fwd")
-    return out.to(hidden.dtype)
+        ws = _ws(_lib.load().moe_mx4_experts_workspace_bytes(f32, T, H, k, E, I), hidden.device)
+        call("moe_mx4_experts", ptr(x), f32, ptr(ids), ptr(w), T, H, k, E, I, *map(ptr, weights), ptr(out), ptr(ws),
+             ws.numel(), _stream(hidden), tag="mx4_experts")
+    return out
 
 
 @mx4_experts.register_fake
