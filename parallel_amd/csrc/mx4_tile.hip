@@ -50,19 +50,23 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
   constexpr int kB = BM * 128, kStage = kB + kTileN * 128;
   constexpr int kScaleWaves = (BM + kTileN) / 64;      // waves that fetch scales, 64 rows each: A's, then B's
   constexpr int kScales = kScaleWaves * 1024, kBs = BM * 16;
+  // Scale slots: a fetch serves two stages, so where a tile has an even number of them two slots do for a DMA cursor
+  // two stages ahead; otherwise one per stage.
+  constexpr int kSlots = STAGES * (kStage + kScales) <= 160 * 1024 ? STAGES : 2;
   constexpr int kStores = EPI == MX4_SWIGLU ? MT : EPI == MX4_PLAIN_F32 ? 4 * MT : 2 * MT;  // store instructions per wave and tile
   // 16-row tiles between whose products the next stage's DMA is fired: a ring of two needs it early.
   constexpr int kFire = STAGES == 2 ? MT / 2 : MT;
-  static_assert(kScaleWaves <= kTileWaves && STAGES * (kStage + kScales) <= 160 * 1024, "LDS");
+  static_assert(kScaleWaves <= kTileWaves && STAGES <= 3 && STAGES * kStage + kSlots * kScales <= 160 * 1024, "LDS");
   static_assert((STAGES - 2) * LPW + kStores < 64, "vmcnt range");
-  __shared__ __attribute__((aligned(1024))) char ring[STAGES * (kStage + kScales)];  // the stages, then their scales
+  __shared__ __attribute__((aligned(1024))) char ring[STAGES * kStage + kSlots * kScales];  // the stages, then their scales
 
   const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave & 1, wn = wave >> 1;
   const int64_t wide = GLU ? 2 * static_cast<int64_t>(p.N) : p.N;
   const uint32_t half_k = static_cast<uint32_t>(p.K) / 2, pitch = static_cast<uint32_t>(mx4_pitch(p.K));
-  const int blocks = p.K / 32, nk = (p.K + 255) / 256;
+  const int blocks = p.K / 32, deep = (p.K + 255) / 256;
+  const int nk = kSlots < STAGES ? (deep + 1) / 2 * 2 : deep;  // stages per tile (the last may lie past K)
 
   int total = 0;
   each_groups(p, [&](int, int, int cnt) {
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
     if (dk & 1) return;
     if (wave < kScaleWaves)
       dma16(rs, s_off + 8u * dk, __builtin_amdgcn_readfirstlane(lds0 + STAGES * kStage + scales_to * kScales + 1024 * wave));
-    scales_to = scales_to + 1 == STAGES ? 0 : scales_to + 1;
+    scales_to = scales_to + 1 == kSlots ? 0 : scales_to + 1;
   };
   auto advance = [&]() __attribute__((always_inline)) {
     if (++dk == nk) seek();
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
       for (int n = i * LPW / kFire; i < kFire && n < (i + 1) * LPW / kFire; ++n) fire(n, to);
     }
     advance();
-    if ((k & 1) || k + 1 == nk) scales_at = scales_at + 1 == STAGES ? 0 : scales_at + 1;
+    if ((k & 1) || k + 1 == nk) scales_at = scales_at + 1 == kSlots ? 0 : scales_at + 1;
   };
   // The tile's results: lane l holds row 16 (wm + 2 i) + l % 16, and of the wave's columns 32 (j / 2) + 8 q + 4 (j %
   // 2) .. + 3 in acc[i][j], or gate and up of act columns 8 q + 4 h .. + 3 in acc[i][2 h] and [2 h + 1].
@@ -337,7 +341,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
       wait_lgkmcnt0();               // this wave's reads of the stage before are done
       __builtin_amdgcn_s_barrier();  // every wave's share landed, and all have left the stage the DMA turns to
       asm volatile("" ::: "memory");
-      multiply(ring + at * kStage, k, t.rows, lds0 + (at ? at - 1 : STAGES - 1) * kStage);
+      multiply(ring + at * kStage, k, k < deep ? t.rows : 0, lds0 + (at ? at - 1 : STAGES - 1) * kStage);
       ++since;
       at = at + 1 == STAGES ? 0 : at + 1;
     }
@@ -371,7 +375,7 @@ int launch(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name) {
 
 int mx4_tile(const Mx4Gemm& p, int epi, int bm, hipStream_t stream, const char* name) {
   return bm <= 64 ? launch<64, 3>(p, epi, stream, name)
-                  : bm <= 128 ? launch<128, 2>(p, epi, stream, name) : launch<256, 2>(p, epi, stream, name);
+                  : bm <= 128 ? launch<128, 3>(p, epi, stream, name) : launch<256, 2>(p, epi, stream, name);
 }
 
 }  // namespace moe
