@@ -206,7 +206,8 @@ int moe_rmsnorm_bwd(const void* dx, const void* dx2, const void* h,
  *   r = rsqrt(mean(h^2) + eps);  hidden = h, x = h * r * gamma, rounded once each.
  * gate_kind: 0 no gate (g = 1, gate NULL), 1 one g per row (gate[T]), 2 one per
  * column (gate[H]), 3 one per element (gate[T,H]).  All operands bf16, or all
- * f32 with is_f32; rstd_y[T] (written with post only) and rstd[T] are f32.
+ * f32 with is_f32; rstd_y[T] (written with post only) and rstd[T] are f32,
+ * either may be NULL (the backward needs them).
  * H a multiple of 8, at most 8192.  For eps = 1e-6, equal scales of 1, no post
  * and no gate, hidden and x are the sum and the norm of
  * TF/models/qwen3_moe/modeling_qwen3_moe.py:340-345 with one rounding. */

@@ -36,6 +36,7 @@ __device__ __forceinline__ float mx4_act(float g, float u) {
 struct Mx4Gemm {
   const uint8_t *a, *a_scales;  // [a_rows, K]
   const int32_t* row_index;     // row r of the product reads row row_index[r] / row_div of A (null: row r)
+  const int64_t* ids;           // few-row kernel, instead of offs and row_index: row r's group, reading row r / row_div
   int row_div, a_rows;
   uint32_t div_magic, div_shift;  // x / row_div = x * div_magic >> div_shift for 0 <= x < 2^31
   const uint8_t *w, *w_scales;  // [G][N, K], or with swiglu [G][2 N, K]: gate rows, then up rows

@@ -15,6 +15,8 @@
 // gate and up of 8 rows of 8 groups, 2048 x 768, 6.7 against 11.2 us (6.7 MB of
 // weights: launch and latency), of 32 rows of 28 groups 13.7 against 13.4; one
 // group's 32 rows x 2048 x 2048 6.8 against 10.5, its 256 rows 21.6 against 11.5.
+// With `ids` every row is a tile of its own in the order the rows come, and no
+// sort or search for it: the experts of a few tokens share none to speak of.
 #include "mx4.h"
 
 namespace moe {
@@ -29,7 +31,16 @@ __global__ __launch_bounds__(kFewWaves * kWave) void mx4_few_kernel(const Mx4Gem
   const int lane = threadIdx.x & (kWave - 1), i16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Mx4Tile t;
-  if (!mx4_find_tile<16>(p, n_tiles, blockIdx.x, t)) return;  // the whole block
+  if (p.ids) {
+    t.r0 = blockIdx.x / n_tiles;
+    t.n = blockIdx.x - t.r0 * n_tiles;
+    t.rows = 1;
+    const int64_t g = p.ids[t.r0];
+    if (g < 0 || g >= p.G) return;  // the whole block
+    t.g = static_cast<int>(g);
+  } else if (!mx4_find_tile<16>(p, n_tiles, blockIdx.x, t)) {
+    return;
+  }
   const int n0 = t.n * kCols;
   const int64_t wide = GLU ? 2 * static_cast<int64_t>(p.N) : p.N;
   const uint32_t half_k = static_cast<uint32_t>(p.K) / 2, pitch = static_cast<uint32_t>(mx4_pitch(p.K));
@@ -41,7 +52,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void mx4_few_kernel(const Mx4Gem
   // The lane's rows of the operands (row 0, and nothing read, where there is none).
   bool a_in = i16 < t.rows, w_in[NT];
   int src = t.r0 + (a_in ? i16 : 0);
-  if (p.row_index) src = mx4_source_row(p, p.row_index[src]);
+  if (p.ids || p.row_index) src = mx4_source_row(p, p.ids ? src : p.row_index[src]);
   a_in = a_in && src >= 0 && src < p.a_rows;
   const uint32_t a_row = a_in ? src : 0;
   uint32_t w_row[NT];
@@ -164,9 +175,9 @@ __global__ __launch_bounds__(kFewWaves * kWave) void mx4_few_kernel(const Mx4Gem
 
 int mx4_few(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name) {
   const int64_t n_tiles = mx4_few_columns(p.N, epi);
-  const int64_t most = mx4_most_tiles(p.rows, p.G, 16) * n_tiles;
+  const int64_t most = (p.ids ? p.rows : mx4_most_tiles(p.rows, p.G, 16)) * n_tiles;
   MOE_REQUIRE(most < (1ll << 30), MOE_ERR_UNSUPPORTED, "%s: too many tiles", name);
-  const dim3 grid(static_cast<unsigned>((most + 7) / 8 * 8)), block(kFewWaves * kWave);
+  const dim3 grid(static_cast<unsigned>(p.ids ? most : (most + 7) / 8 * 8)), block(kFewWaves * kWave);
   const int n = static_cast<int>(n_tiles);
   if (epi == MX4_PLAIN)
     hipLaunchKernelGGL((mx4_few_kernel<MX4_PLAIN>), grid, block, 0, stream, p, n);

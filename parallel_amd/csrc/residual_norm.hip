@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(const RnF
   float ry = 1.0f;
   if (p.post) {
     ry = rsqrtf(row_sum(ss, 0.0f).x * inv_h + p.eps);
-    if (lane == 0) p.rstd_y[t] = ry;
+    if (lane == 0 && p.rstd_y) p.rstd_y[t] = ry;
   }
   const float gt = p.gate_kind == kGateToken ? rn_load1(static_cast<const E*>(p.gate) + t) : 1.0f;
   const E* gr = static_cast<const E*>(p.gate) + (p.gate_kind == kGateFull ? base : 0);
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(const RnF
     }
   }
   const float r = rsqrtf(row_sum(ss, 0.0f).x * inv_h + p.eps);
-  if (lane == 0) p.rstd[t] = r;
+  if (lane == 0 && p.rstd) p.rstd[t] = r;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int c = lane + i * kLanes;
@@ -181,32 +181,34 @@ struct RnBwd {
   float* partials;  // [d_gamma, then d_post if post, then d_gate if per channel][parts][H]
 };
 
-// WHOLE: with post or a gate; without them only the plain sum's registers are kept.
-template <class E, int NC, int WPR, bool WHOLE>
+// EXTRA: 0 the plain sum, whose registers are all it keeps; 1 with post or a gate; 2 with a gate per channel.
+template <class E, int NC, int WPR, int EXTRA>
 __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnBwd p) {
   __shared__ float2 slots[2][4];
   RowSum<WPR> row_sum{slots, 0};
   constexpr int kLanes = WPR * kWave;
+  constexpr bool WHOLE = EXTRA > 0, channel = EXTRA == 2;
   const int lane = threadIdx.x % kLanes;
   const int part = blockIdx.x * (kRnThreads / kLanes) + threadIdx.x / kLanes;
   if (part >= p.parts) return;
   const int n = p.H / 8;
   const float inv_h = 1.0f / static_cast<float>(p.H);
-  const bool post = WHOLE && p.post, channel = WHOLE && p.gate_kind == kGateChannel;
-  float sum_gamma[NC][8], sum_post[WHOLE ? NC : 1][8], sum_gate[WHOLE ? NC : 1][8];
+  const bool post = WHOLE && p.post;
+  float sum_gamma[NC][8], sum_post[WHOLE ? NC : 1][8], sum_gate[channel ? NC : 1][8];
 #pragma unroll
   for (int i = 0; i < NC; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       sum_gamma[i][e] = 0.0f;
-      if constexpr (WHOLE) sum_post[i][e] = sum_gate[i][e] = 0.0f;
+      if constexpr (WHOLE) sum_post[i][e] = 0.0f;
+      if constexpr (channel) sum_gate[i][e] = 0.0f;
     }
   for (int t = part; t < p.T; t += p.parts) {  // the same count for every wave of a row: barriers match
     const int64_t base = static_cast<int64_t>(t) * p.H;
     const float r = p.rstd[t], ry = post ? p.rstd_y[t] : 1.0f;
     const float gt = WHOLE && p.gate_kind == kGateToken ? rn_load1(static_cast<const E*>(p.gate) + t) : 1.0f;
     const E* gr = static_cast<const E*>(p.gate) + (p.gate_kind == kGateFull ? base : 0);
-    float yv[NC][8], h[NC][8], dx[NC][8], dh[NC][8];
+    float yv[NC][8], h[NC][8], dh[NC][8];
     float dot = 0.0f;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -214,12 +216,12 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnB
       if (c < n) {
         rn_load8(static_cast<const E*>(p.y) + base + 8 * c, yv[i]);
         rn_load8(static_cast<const E*>(p.residual) + base + 8 * c, h[i]);
-        if (p.d_x) rn_load8(static_cast<const E*>(p.d_x) + base + 8 * c, dx[i]);
+        float w[8], g[8], v[8], dx[8];
+        if (p.d_x) rn_load8(static_cast<const E*>(p.d_x) + base + 8 * c, dx);
         if (p.d_hidden) rn_load8(static_cast<const E*>(p.d_hidden) + base + 8 * c, dh[i]);
         else
 #pragma unroll
           for (int e = 0; e < 8; ++e) dh[i][e] = 0.0f;
-        float w[8], g[8], v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = yv[i][e];
         if constexpr (WHOLE) {
@@ -243,9 +245,9 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnB
           rn_load8(static_cast<const E*>(p.gamma) + 8 * c, w);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            sum_gamma[i][e] += dx[i][e] * h[i][e] * r;
-            dx[i][e] *= w[e];
-            dot += dx[i][e] * h[i][e];
+            sum_gamma[i][e] += dx[e] * h[i][e] * r;
+            dot += dx[e] * w[e] * h[i][e];
+            dh[i][e] += r * (dx[e] * w[e]);
           }
         }
       }
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnB
       for (int i = 0; i < NC; ++i)
         if (lane + i * kLanes < n)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dh[i][e] += r * dx[i][e] - k * h[i][e];
+          for (int e = 0; e < 8; ++e) dh[i][e] -= k * h[i][e];
     }
     float dot_y = 0.0f, dot_g = 0.0f;
 #pragma unroll
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnB
             const float q = post ? yv[i][e] * ry : yv[i][e];  // v without post's weight
             o[e] = dh[i][e] * (post ? q * w[e] : q);          // the gate's gradient
             dot_g += o[e];
-            if (channel) sum_gate[i][e] += o[e];
+            if constexpr (channel) sum_gate[i][e] += o[e];
             const float dz = dh[i][e] * (p.gate_kind >= kGateChannel ? g[e] : gt);
             if (post) {
               sum_post[i][e] += dz * q;
@@ -324,32 +326,35 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnB
       rn_store8(out + 8 * c, sum_gamma[i]);
       if constexpr (WHOLE) {
         if (post) rn_store8(out + kind + 8 * c, sum_post[i]);
-        if (channel) rn_store8(out + (post ? 2 : 1) * kind + 8 * c, sum_gate[i]);
       }
+      if constexpr (channel) rn_store8(out + (post ? 2 : 1) * kind + 8 * c, sum_gate[i]);
     }
   }
 }
 
-// out[j] = sum of column j over the parts: 16 columns per block, 16 threads
-// taking every 16th part each, then the threads' sums in order.
+// out[j] = sum of column j over the parts: 32 columns per block (a line of
+// 128 bytes of each part), 32 threads taking every 32nd part each, then the
+// threads' sums in order.
+constexpr int kRnSumThreads = 1024;
 template <class E>
-__global__ __launch_bounds__(kRnThreads) void residual_norm_sums_kernel(const float* __restrict__ partials, int parts,
-                                                                        int H, E* out0, E* out1, E* out2) {
-  __shared__ float part[16][17];
-  const int col = threadIdx.x & 15, row = threadIdx.x >> 4;
-  const int j = blockIdx.x * 16 + col;
+__global__ __launch_bounds__(kRnSumThreads) void residual_norm_sums_kernel(const float* __restrict__ partials,
+                                                                           int parts, int H, E* out0, E* out1,
+                                                                           E* out2) {
+  __shared__ float part[32][33];
+  const int col = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const int j = blockIdx.x * 32 + col;
   const float* src = partials + static_cast<int64_t>(blockIdx.y) * parts * H + j;
   float acc = 0.0f;
   if (j < H) {
 #pragma unroll 8
-    for (int q = row; q < parts; q += 16) acc += src[static_cast<int64_t>(q) * H];
+    for (int q = row; q < parts; q += 32) acc += src[static_cast<int64_t>(q) * H];
   }
   part[row][col] = acc;
   __syncthreads();
   if (row == 0 && j < H) {
     float s = 0.0f;
 #pragma unroll
-    for (int q = 0; q < 16; ++q) s += part[q][col];
+    for (int q = 0; q < 32; ++q) s += part[q][col];
     E* out = blockIdx.y == 0 ? out0 : blockIdx.y == 1 ? out1 : out2;
     rn_store1(out + j, s);
   }
@@ -381,10 +386,11 @@ int check_rn(const char* what, const void* y, const void* residual, const void* 
 // 512 values; wider rows take four.
 bool wave_rows(int64_t H) { return H <= 512; }
 
-// Row walkers of the backward: at most 1024 blocks (four per CU, so that the
-// loads of one row run beside the sums of another), each a row of partials.
-int64_t rn_parts(int64_t T, int64_t H) {
-  const int64_t most = wave_rows(H) ? 4096 : 1024;
+// Row walkers of the backward, each a row of partials: at most 1024 blocks (the workspace's size), and as many as run
+// at once, so that no block starts when the others end.
+constexpr int64_t kRnBlocks = 1024;
+int64_t rn_parts(int64_t T, int64_t H, int64_t blocks) {
+  const int64_t most = (wave_rows(H) ? 4 : 1) * blocks;
   return T < 1 ? 1 : T < most ? T : most;
 }
 
@@ -406,7 +412,7 @@ extern "C" int moe_residual_norm_fwd(const void* y, const void* residual, const 
   if (rc) return rc;
   MOE_REQUIRE(eps >= 0.0f, MOE_ERR_INVALID, "residual_norm fwd: eps must be non-negative");
   if (T == 0) return MOE_OK;
-  MOE_REQUIRE(hidden && x && rstd && (rstd_y || !post) && aligned16(hidden) && aligned16(x), MOE_ERR_INVALID,
+  MOE_REQUIRE(hidden && x && aligned16(hidden) && aligned16(x), MOE_ERR_INVALID,
               "residual_norm fwd: bad output pointer");
   const RnFwd p{y,      residual, post, gate, gamma, gate_kind, static_cast<int>(T), static_cast<int>(H), branch_scale,
                 residual_scale, eps, hidden, x, rstd_y, rstd};
@@ -423,7 +429,7 @@ extern "C" int moe_residual_norm_fwd(const void* y, const void* residual, const 
 
 extern "C" size_t moe_residual_norm_bwd_workspace_bytes(int64_t T, int64_t H) {
   if (T < 0 || H < 1) return 0;
-  return static_cast<size_t>(3 * rn_parts(T, H)) * static_cast<size_t>(H) * sizeof(float);
+  return static_cast<size_t>(3 * rn_parts(T, H, kRnBlocks)) * static_cast<size_t>(H) * sizeof(float);
 }
 
 extern "C" int moe_residual_norm_bwd(const void* d_hidden, const void* d_x, const void* y, const void* residual,
@@ -449,32 +455,38 @@ extern "C" int moe_residual_norm_bwd(const void* d_hidden, const void* d_x, cons
   const size_t need = moe_residual_norm_bwd_workspace_bytes(T, H);
   MOE_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= need, MOE_ERR_WORKSPACE,
               "residual_norm bwd: workspace %zu < %zu bytes", workspace_bytes, need);
-  const int parts = static_cast<int>(rn_parts(T, H));
-  const RnBwd p{d_hidden, d_x, y, residual, post, gate, gamma, rstd_y, rstd, gate_kind, static_cast<int>(T),
-                static_cast<int>(H), parts, branch_scale, residual_scale, d_y, d_residual, d_gate,
-                static_cast<float*>(workspace)};
+  RnBwd p{d_hidden, d_x, y, residual, post, gate, gamma, rstd_y, rstd, gate_kind, static_cast<int>(T),
+          static_cast<int>(H), 0, branch_scale, residual_scale, d_y, d_residual, d_gate,
+          static_cast<float*>(workspace)};
   rn_dispatch(H, [&](auto nc, auto wpr) {  // (with T == 0 the one walker writes its zero sums)
     constexpr int NC = decltype(nc)::value, WPR = decltype(wpr)::value, per = 4 / WPR;
-    const dim3 grid((parts + per - 1) / per), block(kRnThreads);
-    auto launch = [&](auto e, auto whole) {
-      hipLaunchKernelGGL((residual_norm_bwd_kernel<decltype(e), NC, WPR, decltype(whole)::value>), grid, block, 0,
-                         as_stream(stream), p);
+    auto launch = [&](auto e, auto extra) {
+      const auto kernel = residual_norm_bwd_kernel<decltype(e), NC, WPR, decltype(extra)::value>;
+      const int dev = current_device();
+      const int64_t fit = static_cast<int64_t>(device_cus(dev)) *
+                          cached_blocks_per_cu(dev, reinterpret_cast<const void*>(kernel), kRnThreads, 0);
+      p.parts = static_cast<int>(rn_parts(T, H, fit < kRnBlocks ? fit : kRnBlocks));
+      hipLaunchKernelGGL(kernel, dim3((p.parts + per - 1) / per), dim3(kRnThreads), 0, as_stream(stream), p);
     };
-    const bool whole = post || gate_kind != kGateNone;
-    if (is_f32) whole ? launch(float{}, std::true_type{}) : launch(float{}, std::false_type{});
-    else whole ? launch(bf16_t{}, std::true_type{}) : launch(bf16_t{}, std::false_type{});
+    auto typed = [&](auto e) {
+      if (channel) launch(e, std::integral_constant<int, 2>{});
+      else if (post || gate_kind != kGateNone) launch(e, std::integral_constant<int, 1>{});
+      else launch(e, std::integral_constant<int, 0>{});
+    };
+    if (is_f32) typed(float{});
+    else typed(bf16_t{});
   });
   rc = launch_status("moe_residual_norm_bwd(rows)");
   if (rc) return rc;
-  const dim3 grid(static_cast<unsigned>((H + 15) / 16), 1 + (post ? 1 : 0) + (channel ? 1 : 0));
+  const dim3 grid(static_cast<unsigned>((H + 31) / 32), 1 + (post ? 1 : 0) + (channel ? 1 : 0));
   void* second = post ? d_post : d_gate;
   if (is_f32)
-    hipLaunchKernelGGL((residual_norm_sums_kernel<float>), grid, dim3(kRnThreads), 0, as_stream(stream), p.partials,
-                       parts, static_cast<int>(H), static_cast<float*>(d_gamma), static_cast<float*>(second),
+    hipLaunchKernelGGL((residual_norm_sums_kernel<float>), grid, dim3(kRnSumThreads), 0, as_stream(stream), p.partials,
+                       p.parts, static_cast<int>(H), static_cast<float*>(d_gamma), static_cast<float*>(second),
                        static_cast<float*>(d_gate));
   else
-    hipLaunchKernelGGL((residual_norm_sums_kernel<bf16_t>), grid, dim3(kRnThreads), 0, as_stream(stream), p.partials,
-                       parts, static_cast<int>(H), static_cast<bf16_t*>(d_gamma), static_cast<bf16_t*>(second),
+    hipLaunchKernelGGL((residual_norm_sums_kernel<bf16_t>), grid, dim3(kRnSumThreads), 0, as_stream(stream), p.partials,
+                       p.parts, static_cast<int>(H), static_cast<bf16_t*>(d_gamma), static_cast<bf16_t*>(second),
                        static_cast<bf16_t*>(d_gate));
   return launch_status("moe_residual_norm_bwd(sums)");
 }

@@ -40,6 +40,13 @@ class MX4Tensor:
         ops._check_mx4("MX4Tensor", codes, scales)
         self.codes, self.scales = codes, scales
 
+    @classmethod
+    def _of(cls, codes: Tensor, scales: Tensor) -> "MX4Tensor":
+        """From parts that an operator made."""
+        t = object.__new__(cls)
+        t.codes, t.scales = codes, scales
+        return t
+
     @property
     def shape(self) -> torch.Size:
         return self.codes.shape[:-1] + (2 * self.codes.shape[-1],)
@@ -72,7 +79,7 @@ def quantize_mx4(x: Tensor) -> MX4Tensor:
     A block's scale is the power of two that puts its largest size in [4, 8);
     every value is rounded to the nearest code, halfway to the even one, sizes
     past 6 to 6.  A block that holds an infinity or NaN is NaN throughout."""
-    return MX4Tensor(*ops.run_mx4("mx4_quantize", x))
+    return MX4Tensor._of(*ops.run_mx4("mx4_quantize", x))
 
 
 def mx4_grouped_mm(a: MX4Tensor, w: MX4Tensor, offsets: Tensor) -> Tensor:

@@ -677,23 +677,31 @@ def _check_residual_norm(y, residual, weight, post_weight, gate) -> int:
     return kind
 
 
+def _residual_norm_launch(y, residual, weight, post_weight, gate, branch_scale, residual_scale, eps, rstd_y, rstd):
+    """(hidden, x); rstd_y and rstd are filled where they are given."""
+    kind = _check_residual_norm(y, residual, weight, post_weight, gate)
+    H = y.shape[-1]
+    hidden, x = torch.empty_like(y, memory_format=torch.contiguous_format), torch.empty_like(
+        y, memory_format=torch.contiguous_format)
+    y, residual, weight = _rows16(y), _rows16(residual), _rows16(weight)
+    post_weight, gate = _rows16_opt(post_weight), _rows16_opt(gate)
+    with _device(y):
+        call("moe_residual_norm_fwd", ptr(y), ptr(residual), ptr(post_weight), ptr(gate), kind, ptr(weight),
+             int(y.dtype == torch.float32), y.numel() // H if H else 0, H, branch_scale, residual_scale, eps,
+             ptr(hidden), ptr(x), ptr(rstd_y), ptr(rstd), _stream(y), tag="residual_norm_fwd")
+    return hidden, x
+
+
 @_op("residual_norm_fwd")
 def residual_norm_fwd(y: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None,
                       branch_scale: float, residual_scale: float, eps: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(hidden, x, rstd_y [T] f32 (empty without post_weight), rstd [T] f32): see residual_norm.residual_norm."""
-    kind = _check_residual_norm(y, residual, weight, post_weight, gate)
-    H = y.shape[-1]
-    T = y.numel() // H if H else 0
-    f32 = dict(dtype=torch.float32, device=y.device)
-    hidden = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    x = torch.empty(y.shape, dtype=y.dtype, device=y.device)
-    rstd_y = torch.empty(0 if post_weight is None else T, **f32)
-    rstd = torch.empty(T, **f32)
-    y, residual, weight, post_weight, gate = map(_rows16_opt, (y, residual, weight, post_weight, gate))
-    with _device(y):
-        call("moe_residual_norm_fwd", ptr(y), ptr(residual), ptr(post_weight), ptr(gate), kind, ptr(weight),
-             int(y.dtype == torch.float32), T, H, branch_scale, residual_scale, eps, ptr(hidden), ptr(x), ptr(rstd_y),
-             ptr(rstd), _stream(y), tag="residual_norm_fwd")
+    _check_residual_norm(y, residual, weight, post_weight, gate)
+    T = y.numel() // max(1, y.shape[-1])
+    rstd_y = torch.empty(0 if post_weight is None else T, dtype=torch.float32, device=y.device)
+    rstd = torch.empty(T, dtype=torch.float32, device=y.device)
+    hidden, x = _residual_norm_launch(y, residual, weight, post_weight, gate, branch_scale, residual_scale, eps,
+                                      rstd_y, rstd)
     return hidden, x, rstd_y, rstd
 
 
@@ -766,8 +774,15 @@ def _residual_norm_backward(ctx, d_hidden, d_x, _d_rstd_y, _d_rstd):
 
 
 residual_norm_fwd.register_autograd(_residual_norm_backward, setup_context=_residual_norm_setup)
-run_residual_norm_fwd = _eager_route("residual_norm_fwd", residual_norm_fwd, _residual_norm_setup,
-                                     _residual_norm_backward)
+_residual_norm_route = _eager_route("residual_norm_fwd", residual_norm_fwd, _residual_norm_setup,
+                                    _residual_norm_backward)
+
+
+def run_residual_norm(*args) -> tuple[Tensor, Tensor]:
+    """(hidden, x) of residual_norm_fwd's arguments; without gradients nothing is kept for them."""
+    if _plain_eager(args) and not _wants_grad(args):
+        return _residual_norm_launch(*args, None, None)
+    return _residual_norm_route(*args)[:2]
 
 
 # ------------------------------------------- 4-bit microscaled operands (mx4)
@@ -792,11 +807,6 @@ def _check_mx4(name: str, codes: Tensor, scales: Tensor) -> int:
         raise ValueError(f"{name}: scales {tuple(scales.shape)} do not match codes {tuple(codes.shape)}: rows of {K} "
                          f"values have {mx4_pitch(K)} scale bytes")
     return K
-
-
-def _refuse_gradients(what: str, *tensors: Tensor) -> None:
-    if _wants_grad(tensors):
-        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
 @_op("mx4_quantize")
@@ -944,8 +954,11 @@ def _(hidden, top_k_index, top_k_weights, gate_up_codes, gate_up_scales, down_co
 
 def run_mx4(name: str, *args):
     """An mx4 op on tensors, with its refusal of gradients."""
-    _refuse_gradients(name, *args)
-    return _direct(name, *args)
+    if _wants_grad(args):
+        raise ValueError(f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+    if _plain_eager(args):
+        return _kernels[name](*args)
+    return getattr(torch.ops.parallel_amd, name)(*args)
 
 
 # ------------------------------------------------------------------ permute

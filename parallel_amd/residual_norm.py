@@ -41,6 +41,5 @@ def residual_norm(
     The arithmetic is fp32 and rounds each output once (x is normed from the
     unrounded sum).  Gradients reach every tensor; the scales and eps are
     numbers, not differentiated."""
-    hidden, x, _, _ = ops.run_residual_norm_fwd(y, residual, weight, post_weight, gate, float(branch_scale),
-                                                float(residual_scale), float(eps))
-    return hidden, x
+    return ops.run_residual_norm(y, residual, weight, post_weight, gate, float(branch_scale), float(residual_scale),
+                                 float(eps))

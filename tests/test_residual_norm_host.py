@@ -38,7 +38,7 @@ def test_c_entry_points_check_their_arguments():
 
     assert fwd(T=0, y=None, x=None) == _lib.MOE_OK  # nothing to do, and no HIP call
     for bad in (dict(y=None), dict(gamma=None), dict(kind=4), dict(kind=1), dict(T=-1), dict(T=1 << 31), dict(eps=-1.0),
-                dict(x=None), dict(y=b + 2), dict(x=b + 8), dict(post=b), dict(gamma=b + 4)):
+                dict(x=None), dict(y=b + 2), dict(x=b + 8), dict(post=b + 8), dict(gamma=b + 4)):
         assert fwd(**bad) == _lib.MOE_ERR_INVALID, bad
     for bad in (dict(H=12), dict(H=0), dict(H=8200)):
         assert fwd(**bad) == _lib.MOE_ERR_UNSUPPORTED, bad
