@@ -114,12 +114,15 @@ def _eager_route(name: str, op, setup, backward):
     fn = type(f"_{name}", (torch.autograd.Function,),
               {"forward": staticmethod(forward), "backward": staticmethod(backward)})
 
+    # Function.apply's own work is for functorch transforms, none of which is active on this route.
+    apply = super(torch.autograd.Function, fn).apply
+
     def route(*args):
         if not _plain_eager(args):
             return op(*args)
         if not _wants_grad(args):
             return kernels(*args)
-        return fn.apply(*args, *defaults[len(args):])  # the backward returns one gradient per parameter
+        return apply(*args, *defaults[len(args):])  # the backward returns one gradient per parameter
 
     return route
 
@@ -677,32 +680,31 @@ def _check_residual_norm(y, residual, weight, post_weight, gate) -> int:
     return kind
 
 
-def _residual_norm_launch(y, residual, weight, post_weight, gate, branch_scale, residual_scale, eps, rstd_y, rstd):
-    """(hidden, x); rstd_y and rstd are filled where they are given."""
+def _residual_norm_launch(y, residual, weight, post_weight, gate, branch_scale, residual_scale, eps, keep):
+    """(hidden, x), and with ``keep`` rstd_y [T] f32 (empty without post_weight) and rstd [T] f32."""
     kind = _check_residual_norm(y, residual, weight, post_weight, gate)
     H = y.shape[-1]
+    T = y.numel() // H if H else 0
+    rstd_y = rstd = None
+    if keep:
+        rstd = torch.empty(T, dtype=torch.float32, device=y.device)
+        rstd_y = torch.empty(0 if post_weight is None else T, dtype=torch.float32, device=y.device)
     hidden, x = torch.empty_like(y, memory_format=torch.contiguous_format), torch.empty_like(
         y, memory_format=torch.contiguous_format)
     y, residual, weight = _rows16(y), _rows16(residual), _rows16(weight)
     post_weight, gate = _rows16_opt(post_weight), _rows16_opt(gate)
     with _device(y):
         call("moe_residual_norm_fwd", ptr(y), ptr(residual), ptr(post_weight), ptr(gate), kind, ptr(weight),
-             int(y.dtype == torch.float32), y.numel() // H if H else 0, H, branch_scale, residual_scale, eps,
-             ptr(hidden), ptr(x), ptr(rstd_y), ptr(rstd), _stream(y), tag="residual_norm_fwd")
-    return hidden, x
+             int(y.dtype == torch.float32), T, H, branch_scale, residual_scale, eps, ptr(hidden), ptr(x), ptr(rstd_y),
+             ptr(rstd), _stream(y), tag="residual_norm_fwd")
+    return (hidden, x, rstd_y, rstd) if keep else (hidden, x)
 
 
 @_op("residual_norm_fwd")
 def residual_norm_fwd(y: Tensor, residual: Tensor, weight: Tensor, post_weight: Tensor | None, gate: Tensor | None,
                       branch_scale: float, residual_scale: float, eps: float) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """(hidden, x, rstd_y [T] f32 (empty without post_weight), rstd [T] f32): see residual_norm.residual_norm."""
-    _check_residual_norm(y, residual, weight, post_weight, gate)
-    T = y.numel() // max(1, y.shape[-1])
-    rstd_y = torch.empty(0 if post_weight is None else T, dtype=torch.float32, device=y.device)
-    rstd = torch.empty(T, dtype=torch.float32, device=y.device)
-    hidden, x = _residual_norm_launch(y, residual, weight, post_weight, gate, branch_scale, residual_scale, eps,
-                                      rstd_y, rstd)
-    return hidden, x, rstd_y, rstd
+    return _residual_norm_launch(y, residual, weight, post_weight, gate, branch_scale, residual_scale, eps, True)
 
 
 @residual_norm_fwd.register_fake
@@ -712,32 +714,39 @@ def _(y, residual, weight, post_weight, gate, branch_scale, residual_scale, eps)
             y.new_empty(0 if post_weight is None else T, dtype=torch.float32), y.new_empty(T, dtype=torch.float32))
 
 
+def _residual_norm_bwd_launch(d_hidden, d_x, y, residual, weight, post_weight, gate, rstd_y, rstd, branch_scale,
+                              residual_scale):
+    """The op's gradients, None where there is none (d_y: also where it equals d_residual)."""
+    kind = _gate_kind(y, gate)
+    H = y.shape[-1]
+    T = y.numel() // H if H else 0
+    dev, dt = y.device, y.dtype
+    d_residual = torch.empty(y.shape, dtype=dt, device=dev)
+    d_y = None if _one_input_gradient(post_weight, gate, branch_scale, residual_scale) else torch.empty_like(d_residual)
+    d_weight = torch.empty(H, dtype=dt, device=dev)
+    d_post = None if post_weight is None else torch.empty_like(d_weight)
+    d_gate = None if gate is None else torch.empty(gate.shape, dtype=dt, device=dev)
+    d_hidden, d_x = (None if d is None else _rows16(d if d.dtype == dt else d.to(dt)) for d in (d_hidden, d_x))
+    y, residual, weight = _rows16(y), _rows16(residual), _rows16(weight)
+    post_weight, gate = _rows16_opt(post_weight), _rows16_opt(gate)
+    with _device(y):
+        ws = _ws(_lib.load().moe_residual_norm_bwd_workspace_bytes(T, H), dev)
+        call("moe_residual_norm_bwd", ptr(d_hidden), ptr(d_x), ptr(y), ptr(residual), ptr(post_weight), ptr(gate),
+             kind, ptr(weight), ptr(rstd_y), ptr(rstd), int(dt == torch.float32), T, H, branch_scale, residual_scale,
+             ptr(d_y), ptr(d_residual), ptr(d_post), ptr(d_gate), ptr(d_weight), ptr(ws), ws.numel(), _stream(y),
+             tag="residual_norm_bwd")
+    return d_y, d_residual, d_weight, d_post, d_gate
+
+
 @_op("residual_norm_bwd")
 def residual_norm_bwd(d_hidden: Tensor | None, d_x: Tensor | None, y: Tensor, residual: Tensor, weight: Tensor,
                       post_weight: Tensor | None, gate: Tensor | None, rstd_y: Tensor, rstd: Tensor,
                       branch_scale: float, residual_scale: float) -> tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """(d_y, d_residual, d_weight, d_post_weight, d_gate) of residual_norm_fwd; empty where there is no such
     gradient, and d_y also where it equals d_residual (no post_weight, no gate, equal scales)."""
-    kind = _gate_kind(y, gate)
-    H = y.shape[-1]
-    T = y.numel() // H if H else 0
-    dev, dt = y.device, y.dtype
-    one = _one_input_gradient(post_weight, gate, branch_scale, residual_scale)
-    d_residual = torch.empty(y.shape, dtype=dt, device=dev)
-    d_y = torch.empty(0 if one else y.shape, dtype=dt, device=dev)
-    d_weight = torch.empty(H, dtype=dt, device=dev)
-    d_post = torch.empty(0 if post_weight is None else H, dtype=dt, device=dev)
-    d_gate = torch.empty(0 if gate is None else gate.shape, dtype=dt, device=dev)
-    d_hidden, d_x = (None if d is None else _rows16(d.to(dt)) for d in (d_hidden, d_x))
-    y, residual, weight, post_weight, gate = map(_rows16_opt, (y, residual, weight, post_weight, gate))
-    with _device(y):
-        ws = _ws(_lib.load().moe_residual_norm_bwd_workspace_bytes(T, H), dev)
-        call("moe_residual_norm_bwd", ptr(d_hidden), ptr(d_x), ptr(y), ptr(residual), ptr(post_weight), ptr(gate),
-             kind, ptr(weight), ptr(rstd_y), ptr(rstd), int(dt == torch.float32), T, H, branch_scale, residual_scale,
-             None if one else ptr(d_y), ptr(d_residual), None if post_weight is None else ptr(d_post),
-             None if gate is None else ptr(d_gate), ptr(d_weight), ptr(ws), ws.numel(), _stream(y),
-             tag="residual_norm_bwd")
-    return d_y, d_residual, d_weight, d_post, d_gate
+    grads = _residual_norm_bwd_launch(d_hidden, d_x, y, residual, weight, post_weight, gate, rstd_y, rstd, branch_scale,
+                                      residual_scale)
+    return tuple(y.new_empty(0) if g is None else g for g in grads)
 
 
 def _one_input_gradient(post_weight, gate, branch_scale: float, residual_scale: float) -> bool:
@@ -764,9 +773,12 @@ def _residual_norm_setup(ctx, inputs, output):
 def _residual_norm_backward(ctx, d_hidden, d_x, _d_rstd_y, _d_rstd):
     if d_hidden is None and d_x is None:
         return (None,) * 8
-    y, residual, weight, post_weight, gate, rstd_y, rstd = ctx.saved_tensors
-    d_y, d_res, d_w, d_post, d_gate = _direct("residual_norm_bwd", d_hidden, d_x, y, residual, weight, post_weight,
-                                              gate, rstd_y, rstd, *ctx.scales)
+    args = (d_hidden, d_x, *ctx.saved_tensors, *ctx.scales)
+    if _plain_eager(args) and not _wants_grad(args):
+        d_y, d_res, d_w, d_post, d_gate = _residual_norm_bwd_launch(*args)
+    else:
+        d_y, d_res, d_w, d_post, d_gate = torch.ops.parallel_amd.residual_norm_bwd(*args)
+    post_weight, gate = args[5:7]
     if _one_input_gradient(post_weight, gate, *ctx.scales):
         d_y = d_res
     return (d_y, d_res, d_w, None if post_weight is None else d_post, None if gate is None else d_gate,
@@ -781,7 +793,7 @@ _residual_norm_route = _eager_route("residual_norm_fwd", residual_norm_fwd, _res
 def run_residual_norm(*args) -> tuple[Tensor, Tensor]:
     """(hidden, x) of residual_norm_fwd's arguments; without gradients nothing is kept for them."""
     if _plain_eager(args) and not _wants_grad(args):
-        return _residual_norm_launch(*args, None, None)
+        return _residual_norm_launch(*args, False)
     return _residual_norm_route(*args)[:2]
 
 
