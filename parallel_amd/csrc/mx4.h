@@ -32,6 +32,14 @@ __device__ __forceinline__ float mx4_act(float g, float u) {
   return g * u * __builtin_amdgcn_rcpf(1.0f + e);
 }
 
+// The largest of the four lane quarters' values, in every quarter (register swaps of 16- and 32-lane rows).
+__device__ __forceinline__ uint32_t quarters_max(uint32_t v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  v = max(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  return max(b[0], b[1]);
+}
+
 // One product launch.
 struct Mx4Gemm {
   const uint8_t *a, *a_scales;  // [a_rows, K]

@@ -152,8 +152,7 @@ __global__ __launch_bounds__(kFewWaves * kWave) void mx4_few_kernel(const Mx4Gem
       uint32_t top = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(act[e / 4][e % 4]) & 0x7fffffffu);
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+      top = quarters_max(top);
       const uint32_t s = mx4_scale(top);
       const float f = mx4_scale_f(s);
       if (in && n0 < p.N) {

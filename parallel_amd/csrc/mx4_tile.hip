@@ -296,8 +296,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
           uint32_t top = 0;
 #pragma unroll
           for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(act[e]) & 0x7fffffffu);
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16)));
-          top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32)));
+          top = quarters_max(top);
           const uint32_t s = mx4_scale(top);
           const float f = mx4_scale_f(s);
           uint32_t c = 0;
