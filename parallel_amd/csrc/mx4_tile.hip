@@ -252,6 +252,13 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
   // The tile's results: lane l holds row 16 (wm + 2 i) + l % 16, and of the wave's columns 32 (j / 2) + 8 q + 4 (j %
   // 2) .. + 3 in acc[i][j], or gate and up of act columns 8 q + 4 h .. + 3 in acc[i][2 h] and [2 h + 1].
   auto store = [&](const Mx4Tile& t) __attribute__((always_inline)) {
+    // An offset past the compiler's sight, so that it does not branch on its choice and split the store: the waits
+    // count one store instruction for each below.
+    auto at = [](bool in, uint32_t off) __attribute__((always_inline)) {
+      uint32_t v = in ? off : kOOB;
+      asm("" : "+v"(v));
+      return v;
+    };
     auto put16 = [](__amdgpu_buffer_rsrc_t rs, uint32_t off, const float (&o)[8]) {
       __builtin_amdgcn_raw_buffer_store_b128(u32x4_t{pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
                                                      pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7])}, rs, off, 0, 0);
@@ -270,7 +277,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
         for (int j = 0; j < NT; ++j) {
           const uint32_t n = n0 + 32 * (j / 2) + 8 * q + 4 * (j % 2);
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[i][j]), rc,
-                                                 in && n < N ? (row * N + n) * 4u : kOOB, 0, 0);
+                                                 at(in && n < N, (row * N + n) * 4u), 0, 0);
         }
       } else if constexpr (EPI == MX4_PLAIN) {
 #pragma unroll
@@ -279,7 +286,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
           float o[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] = acc[i][2 * h + e / 4][e % 4];
-          put16(rc, in && n < N ? (row * N + n) * 2u : kOOB, o);
+          put16(rc, at(in && n < N, (row * N + n) * 2u), o);
         }
       } else {
         float act[8];
@@ -287,7 +294,7 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
         for (int e = 0; e < 8; ++e) act[e] = mx4_act(acc[i][2 * (e / 4)][e % 4], acc[i][2 * (e / 4) + 1][e % 4]);
         if constexpr (EPI == MX4_SWIGLU) {
           const uint32_t n = n0 + 8 * q;
-          put16(rc, in && n < N ? (row * N + n) * 2u : kOOB, act);
+          put16(rc, at(in && n < N, (row * N + n) * 2u), act);
         } else {  // quantised from fp32: one rounding, to 4 bits
           const uint32_t out_pitch = static_cast<uint32_t>(mx4_pitch(N));
           const auto rcc = make_rsrc(p.c_codes + static_cast<int64_t>(t.r0) * (N / 2), static_cast<uint32_t>(t.rows) * (N / 2));
@@ -305,9 +312,8 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
           c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[4], act[5], f, 2);
           c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, act[6], act[7], f, 3);
           const bool w = in && n0 < N;
-          __builtin_amdgcn_raw_buffer_store_b32(s == 255u ? 0u : c, rcc, w ? row * (N / 2) + n0 / 2 + 4 * q : kOOB, 0, 0);
-          __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(s), rcs, w && q == 0 ? row * out_pitch + n0 / 32 : kOOB,
-                                               0, 0);
+          __builtin_amdgcn_raw_buffer_store_b32(s == 255u ? 0u : c, rcc, at(w, row * (N / 2) + n0 / 2 + 4 * q), 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(s), rcs, at(w && q == 0, row * out_pitch + n0 / 32), 0, 0);
         }
       }
     }

@@ -34,6 +34,8 @@ class MX4Tensor:
     __slots__ = ("codes", "scales")
 
     def __init__(self, codes: Tensor, scales: Tensor):
+        if not codes.dim() or not scales.dim():
+            raise ValueError("MX4Tensor: codes and scales need a dimension of values")
         K = 2 * codes.shape[-1]
         if scales.shape[-1] * 32 == K and scales.shape[-1] != ops.mx4_pitch(K):
             scales = nn.functional.pad(scales, (0, ops.mx4_pitch(K) - scales.shape[-1]))
@@ -61,7 +63,7 @@ class MX4Tensor:
         return self.scales[..., :self.codes.shape[-1] // 16]
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> Tensor:
-        """The values, exactly, in bfloat16 or float32."""
+        """The values, exactly, in bfloat16 or float32 (infinity past their range)."""
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"4-bit values are given as bfloat16 or float32, not {dtype}")
         return ops.run_mx4("mx4_dequantize", self.codes, self.scales, dtype == torch.float32)

@@ -848,7 +848,7 @@ def _(x):
 
 @_op("mx4_dequantize")
 def mx4_dequantize(codes: Tensor, scales: Tensor, float32: bool) -> Tensor:
-    """The values [..., K] of an mx4 tensor, bfloat16 (exact) or float32."""
+    """The values [..., K] of an mx4 tensor, exactly, in bfloat16 or float32 (infinity past their range)."""
     K = _check_mx4("mx4_dequantize", codes, scales)
     _require_gpu(codes, scales)
     _require_one_device(codes, scales)
@@ -961,7 +961,7 @@ def mx4_experts(hidden: Tensor, top_k_index: Tensor, top_k_weights: Tensor, gate
 
 @mx4_experts.register_fake
 def _(hidden, top_k_index, top_k_weights, gate_up_codes, gate_up_scales, down_codes, down_scales):
-    return torch.empty_like(hidden)
+    return hidden.new_empty(hidden.shape)
 
 
 def run_mx4(name: str, *args):

@@ -153,6 +153,24 @@ def test_grouped_products(counts, N, K):
     within(mx4_swiglu(a, w, offs), act, e, "swiglu")
 
 
+# Mean rows for each kernel: few rows in all; 64-, 128- and 256-row tiles; K with an odd number of 256-value stages,
+# with part of one, and with one; columns past a tile; one or two rows in most tiles; one group with nearly all rows.
+@pytest.mark.parametrize("rows,G,N,K,skew", [
+    (40, 5, 200, 544, 0), (2000, 64, 328, 544, 0), (384, 128, 264, 512, 0), (2600, 64, 520, 96, 0), (1500, 64, 520, 1056, 2),
+    (1000, 8, 328, 544, 0), (1300, 10, 264, 800, 0), (900, 8, 136, 32, 0), (2000, 8, 328, 544, 0), (900, 3, 264, 2080, 0),
+    (5000, 16, 264, 288, 2), (700, 2, 8, 256, 0), (4096, 300, 264, 160, 0),
+])
+def test_every_tile_height(rows, G, N, K, skew):
+    g = gen(rows + K)
+    weight = (torch.arange(G, device=DEV) + 1.0) ** -float(skew)
+    counts = torch.bincount(torch.multinomial(weight, rows, replacement=True, generator=g), minlength=G).tolist()
+    a, av = operand(g, rows, K)
+    w, wv = operand(g, G, 2 * N, K, std=0.1)
+    want, err = O.product(av, wv, counts)
+    within(mx4_grouped_mm(a, w, offsets_of(counts)), want, err, "mm")
+    within(mx4_swiglu(a, w, offsets_of(counts)), *O.swiglu(want, err), "swiglu")
+
+
 @pytest.mark.parametrize("rows,G,N,K", [(3000, 8, 512, 768), (700, 3, 768, 1024), (9000, 64, 256, 256), (130, 128, 96, 1536)])
 def test_larger_products(rows, G, N, K):
     g = gen(rows)
@@ -211,7 +229,7 @@ def layer(g, E, H, I):
 
 
 def experts_oracle(x, idx, wts, guv, dnv):
-    """(out, bound) of the path: quantised tokens, fp32 products, quantised act, bf16 rows, fp32 combine."""
+    """(out, bound) of the path: quantised tokens, fp32 products, quantised act, fp32 or bf16 rows, fp32 combine."""
     E = guv.shape[0]
     xv = O.values(*O.quantize(x))
     T, k = idx.shape
@@ -225,7 +243,8 @@ def experts_oracle(x, idx, wts, guv, dnv):
         mid, far = O.requantize(act, ea)
         y, ey = O.product(mid, dnv[e:e + 1], [t.numel()])
         ey = ey + far @ dnv[e].t().abs()
-        ey = ey + 2.0 ** -8 * (y.abs() + ey)  # the rows are held in bf16
+        if x.dtype == BF and x.shape[0] * k * x.shape[1] > 1 << 22:  # the rows are held in bf16
+            ey = ey + 2.0 ** -8 * (y.abs() + ey)
         wt = wts[t, j].double().unsqueeze(1)
         out.index_add_(0, t, wt * y)
         err.index_add_(0, t, wt.abs() * ey)
@@ -234,7 +253,9 @@ def experts_oracle(x, idx, wts, guv, dnv):
 
 
 @pytest.mark.parametrize("T,H,E,k,I", [(1, 64, 8, 2, 32), (1, 2048, 128, 8, 768), (7, 256, 8, 2, 128), (48, 512, 32, 4, 160),
-                                       (333, 416, 8, 3, 288), (1500, 512, 4, 2, 256), (4096, 256, 16, 2, 96)])
+                                       (333, 416, 8, 3, 288), (1500, 512, 4, 2, 256), (4096, 256, 16, 2, 96),
+                                       (8, 256, 16, 8, 64), (9, 256, 16, 8, 64), (300, 256, 32, 4, 288),
+                                       (100, 512, 64, 4, 320), (3000, 512, 8, 4, 64), (2500, 1056, 64, 2, 160)])
 def test_experts(T, H, E, k, I):
     g = gen(T + H)
     gu, guv, dn, dnv = layer(g, E, H, I)
@@ -262,7 +283,15 @@ def test_experts_routing_corners():
         assert out.dtype == dt
         within(out, *experts_oracle(x.to(dt), idx, wts, guv, dnv))
         assert not out[20].any() and not out[3].any()
+    few = slice(15, 35)  # few enough slots to go without a sort, with sentinels and repeated experts among them
+    within(mx4_experts(x[few], idx[few], wts[few], gu, dn), *experts_oracle(x[few], idx[few], wts[few], guv, dnv))
+    neg = idx[few].clone()
+    neg[3, 1] = -1
+    out = mx4_experts(x[few], neg, wts[few], gu, dn)
+    within(out, *experts_oracle(x[few], neg, wts[few], guv, dnv))
     x[6, 17] = float("inf")
+    few = mx4_experts(x[:9], idx[:9], wts[:9], gu, dn)
+    assert torch.isnan(few[6]).all() and torch.isfinite(few[:6]).all() and torch.isfinite(few[7:]).all()
     bad = mx4_experts(x, idx, wts, gu, dn)
     assert torch.isnan(bad[6]).all() and torch.isfinite(bad[torch.arange(T, device=DEV) != 6]).all()
     assert mx4_experts(x[:0], idx[:0], wts[:0], gu, dn).shape == (0, H)
