@@ -54,8 +54,8 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
   // two stages ahead; otherwise one per stage.
   constexpr int kSlots = STAGES * (kStage + kScales) <= 160 * 1024 ? STAGES : 2;
   constexpr int kStores = EPI == MX4_SWIGLU ? MT : EPI == MX4_PLAIN_F32 ? 4 * MT : 2 * MT;  // store instructions per wave and tile
-  // 16-row tiles between whose products the next stage's DMA is fired: a ring of two needs it early.
-  constexpr int kFire = STAGES == 2 ? MT / 2 : MT;
+  // Groups of products between which the next stage's DMA is fired: a ring of two needs it early.
+  constexpr int kFire = STAGES == 2 ? MT : 2 * MT;
   static_assert(kScaleWaves <= kTileWaves && STAGES <= 3 && STAGES * kStage + kSlots * kScales <= 160 * 1024, "LDS");
   static_assert((STAGES - 2) * LPW + kStores < 64, "vmcnt range");
   __shared__ __attribute__((aligned(1024))) char ring[STAGES * kStage + kSlots * kScales];  // the stages, then their scales
@@ -215,36 +215,38 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
 #pragma unroll
     for (int j = 0; j < NT; ++j) 
       sw[j] = *reinterpret_cast<const uint16_t*>(sc + kBs + (64 * wn + 16 * j + i16) * 16) & keep;
-    uint4 w[2][NT];
+    // The products of a stage's first 32-blocks go over all row tiles before those of the second: half of B's
+    // fragments are read while the first half multiplies, and each tile's next fragment a tile ahead.  Tiles
+    // without rows skip their products.
+    uint4 w[2][NT], a[2];
+    uint32_t sa[MT];
+    auto read_b = [&](int s, int j) __attribute__((always_inline)) {
+      w[s][j] = *reinterpret_cast<const uint4*>(st + kB + (b_row + 4 * j) * 128 + (((4 * s + q) ^ swz) << 4));
+    };
+    auto read_a = [&](int n) __attribute__((always_inline)) {
+      const int s = n / MT, r = 16 * (wm + WM * (n % MT));
+      if (s == 0) sa[n] = *reinterpret_cast<const uint16_t*>(sc + (r + i16) * 16) & keep;
+      a[n & 1] = *reinterpret_cast<const uint4*>(st + r * 128 + a_lane + (((4 * s + q) ^ swz) << 4));
+    };
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int j = 0; j < NT; ++j) read_b(0, j);
+    read_a(0);
+#pragma unroll
+    for (int n = 0; n < 2 * MT; ++n) {
+      const int s = n / MT, i = n % MT;
+      if (n + 1 < 2 * MT) read_a(n + 1);
 #pragma unroll
       for (int j = 0; j < NT; ++j)
-        w[s][j] = *reinterpret_cast<const uint4*>(st + kB + (b_row + 4 * j) * 128 + (((4 * s + q) ^ swz) << 4));
-    // The next 16 rows' fragments are read while these are multiplied; tiles
-    // without rows skip their products.
-    uint4 a[2][2];
-    uint32_t sa[2];
-    auto read = [&](int i) __attribute__((always_inline)) {
-      const int r = 16 * (wm + WM * i);
-      sa[i & 1] = *reinterpret_cast<const uint16_t*>(sc + (r + i16) * 16) & keep;
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-        a[i & 1][s] = *reinterpret_cast<const uint4*>(st + r * 128 + a_lane + (((4 * s + q) ^ swz) << 4));
-    };
-    read(0);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      if (i + 1 < MT) read(i + 1);
+        if (s == 0 && j * MT / NT == i) read_b(1, j);
       if (16 * (wm + WM * i) < rows) {  // wave-uniform
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mx4_mfma<0>(w[0][j], a[i & 1][0], acc[i][j], sw[j], sa[i & 1]);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = mx4_mfma<1>(w[1][j], a[i & 1][1], acc[i][j], sw[j], sa[i & 1]);
+        for (int j = 0; j < NT; ++j)
+          acc[i][j] = s == 0 ? mx4_mfma<0>(w[0][j], a[n & 1], acc[i][j], sw[j], sa[i])
+                             : mx4_mfma<1>(w[1][j], a[n & 1], acc[i][j], sw[j], sa[i]);
       }
-      if (i == 0) fire_scales();
+      if (n == 0) fire_scales();
 #pragma unroll
-      for (int n = i * LPW / kFire; i < kFire && n < (i + 1) * LPW / kFire; ++n) fire(n, to);
+      for (int f = n * LPW / kFire; n < kFire && f < (n + 1) * LPW / kFire; ++f) fire(f, to);
     }
     advance();
     if ((k & 1) || k + 1 == nk) scales_at = scales_at + 1 == kSlots ? 0 : scales_at + 1;
