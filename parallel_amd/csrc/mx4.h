@@ -44,7 +44,8 @@ __device__ __forceinline__ uint32_t quarters_max(uint32_t v) {
 struct Mx4Gemm {
   const uint8_t *a, *a_scales;  // [a_rows, K]
   const int32_t* row_index;     // row r of the product reads row row_index[r] / row_div of A (null: row r)
-  const int64_t* ids;           // few-row kernel, instead of offs and row_index: row r's group, reading row r / row_div
+  const int64_t* ids;           // slots, instead of offs and row_index: row r's group, reading row r / row_div
+  const void* x;                // slots: A's rows as they are, bf16 or f32
   int row_div, a_rows;
   uint32_t div_magic, div_shift;  // x / row_div = x * div_magic >> div_shift for 0 <= x < 2^31
   const uint8_t *w, *w_scales;  // [G][N, K], or with swiglu [G][2 N, K]: gate rows, then up rows
@@ -146,6 +147,10 @@ inline int64_t mx4_few_columns(int64_t N, int epi) { return mx4_glu(epi) ? (N + 
 
 // Products of few tiles in all (mx4_few.hip).
 int mx4_few(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name);
+// The experts of a few slots: gate and up (p: rows = T k slots, ids, x, row_div = k, the act rows' mx4 output) and
+// down with the weighted sum (mx4_few.hip).
+int mx4_slots(const Mx4Gemm& up, bool is_f32, const uint8_t* down, const uint8_t* down_scales, const float* weights,
+              int64_t T, int64_t H, int64_t k, void* out, hipStream_t stream);
 // Products of many rows per group in tiles of up to bm (64, 128 or 256) rows (mx4_tile.hip).
 int mx4_tile(const Mx4Gemm& p, int epi, int bm, hipStream_t stream, const char* name);
 

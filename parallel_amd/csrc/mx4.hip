@@ -94,29 +94,22 @@ __global__ __launch_bounds__(kMx4Threads) void mx4_dequantize_kernel(const uint3
   }
 }
 
-// out[t, :] = sum over the token's slots, in slot order, of weight * row (fp32 rows), 8 columns a thread.  The row of
-// a slot is at pos_of_slot, of which offsets[E - 1] hold one, or (pos_of_slot null) at the slot, where its id is one.
+// out[t, :] = sum over the token's slots, in slot order, of weight * row (fp32 rows), 8 columns a thread.
 template <class E>
 __global__ __launch_bounds__(kMx4Threads) void mx4_combine_kernel(const float* __restrict__ y,
                                                                   const int32_t* __restrict__ pos_of_slot,
-                                                                  const int32_t* __restrict__ offsets,
-                                                                  const int64_t* __restrict__ ids, int experts,
+                                                                  const int32_t* __restrict__ offsets, int experts,
                                                                   const float* __restrict__ weights, int H, int k,
                                                                   int per_row, E* __restrict__ out) {
   const int64_t t = blockIdx.x / per_row;
   const int c = (blockIdx.x % per_row) * kMx4Threads + threadIdx.x;
   if (c >= H / 8) return;
-  const int valid = pos_of_slot ? offsets[experts - 1] : 0;
+  const int valid = offsets[experts - 1];
   float o[8] = {};
 #pragma unroll 4
   for (int j = 0; j < k; ++j) {
-    int64_t pos = t * k + j;
-    if (pos_of_slot) {
-      pos = pos_of_slot[pos];
-      if (pos >= valid) continue;  // the slot's expert is elsewhere
-    } else if (ids[pos] < 0 || ids[pos] >= experts) {
-      continue;
-    }
+    const int64_t pos = pos_of_slot[t * k + j];
+    if (pos >= valid) continue;  // the slot's expert is elsewhere
     const float w = weights[t * k + j];
     const float4* row = reinterpret_cast<const float4*>(y + pos * H + 8 * c);
     const float4 a = row[0], b = row[1];
@@ -158,6 +151,15 @@ unsigned pass_blocks(int64_t n8) {
   return static_cast<unsigned>(blocks < 16384 ? blocks : 16384);
 }
 
+// Granlund and Montgomery's multiplier: with l = ceil(log2 d), m = floor(2^(31+l) / d) + 1 divides 31-bit numbers.
+void set_divisor(Mx4Gemm& p, int64_t d) {
+  uint32_t l = 0;
+  while ((1ll << l) < d) ++l;
+  p.row_div = static_cast<int>(d);
+  p.div_magic = static_cast<uint32_t>((1ull << (31 + l)) / static_cast<uint64_t>(d) + 1);
+  p.div_shift = 31 + l;
+}
+
 // Which kernel, from the rows and groups alone (the groups' own counts are on the device).
 // The few-row kernel where it needs at most 512 blocks (16 rows by 64 weight rows each) and groups are small: it
 // is then ahead of 64-row tiles or level (mx4_few.hip has the times).  Tiles of 64, 128 or 256 rows by the mean:
@@ -168,14 +170,13 @@ unsigned pass_blocks(int64_t n8) {
 int mx4_product(const Mx4Gemm& p, int epi, hipStream_t stream, const char* what) {
   const int64_t mean = (static_cast<int64_t>(p.rows) + p.G - 1) / p.G;
   const int64_t groups = p.G < p.rows ? p.G : p.rows;
-  if (p.ids) return mx4_few(p, epi, stream, what);
   if (mean <= 64 && (groups + (p.rows - groups) / 16) * mx4_few_columns(p.N, epi) <= 512)
     return mx4_few(p, epi, stream, what);
   return mx4_tile(p, epi, mean <= 56 ? 64 : mean <= 160 ? 128 : 256, stream, what);
 }
 
 int run_product(const char* what, const void* a, const void* a_scales, int64_t a_rows, const int32_t* row_index,
-                const int64_t* ids, int64_t row_div, const void* w, const void* w_scales, const int32_t* offs, int64_t G, int64_t M,
+                int64_t row_div, const void* w, const void* w_scales, const int32_t* offs, int64_t G, int64_t M,
                 int64_t N, int64_t K, void* c, void* c_codes, void* c_scales, int epi, void* stream) {
   const int64_t wide = mx4_glu(epi) ? 2 * N : N;
   MOE_REQUIRE(G > 0 && M >= 0 && a_rows >= 0 && N > 0 && K > 0 && row_div > 0, MOE_ERR_INVALID, "%s: bad sizes", what);
@@ -188,9 +189,9 @@ int run_product(const char* what, const void* a, const void* a_scales, int64_t a
               MOE_ERR_UNSUPPORTED, "%s: sizes past 32 bits", what);
   MOE_REQUIRE(a_rows * (K / 2) < (1ll << 31) && wide * (K / 2) < (1ll << 31), MOE_ERR_UNSUPPORTED,
               "%s: the activations and each group's weights must stay below 2 GiB", what);
-  MOE_REQUIRE(row_index || ids || a_rows >= M, MOE_ERR_INVALID, "%s: %lld activation rows for %lld", what, (long long)a_rows,
+  MOE_REQUIRE(row_index || a_rows >= M, MOE_ERR_INVALID, "%s: %lld activation rows for %lld", what, (long long)a_rows,
               (long long)M);
-  MOE_REQUIRE(w && w_scales && (offs || ids) && aligned16(w) && aligned8(w_scales), MOE_ERR_INVALID,
+  MOE_REQUIRE(w && w_scales && offs && aligned16(w) && aligned8(w_scales), MOE_ERR_INVALID,
               "%s: bad weight or offsets pointer", what);
   if (M == 0) return MOE_OK;
   MOE_REQUIRE(a && a_scales && aligned16(a) && aligned8(a_scales), MOE_ERR_INVALID, "%s: bad activation pointer", what);
@@ -204,13 +205,7 @@ int run_product(const char* what, const void* a, const void* a_scales, int64_t a
   p.a = static_cast<const uint8_t*>(a);
   p.a_scales = static_cast<const uint8_t*>(a_scales);
   p.row_index = row_index;
-  p.ids = ids;
-  p.row_div = static_cast<int>(row_div);
-  // Granlund and Montgomery's multiplier: with l = ceil(log2 d), m = floor(2^(31+l) / d) + 1 divides 31-bit numbers.
-  uint32_t l = 0;
-  while ((1ll << l) < row_div) ++l;
-  p.div_magic = static_cast<uint32_t>((1ull << (31 + l)) / static_cast<uint64_t>(row_div) + 1);
-  p.div_shift = 31 + l;
+  set_divisor(p, row_div);
   p.a_rows = static_cast<int>(a_rows);
   p.w = static_cast<const uint8_t*>(w);
   p.w_scales = static_cast<const uint8_t*>(w_scales);
@@ -265,7 +260,7 @@ extern "C" int moe_mx4_grouped_gemm(const void* a_codes, const void* a_scales, i
                                     const int32_t* row_index, int64_t row_divisor, const void* w_codes,
                                     const void* w_scales, const int32_t* offs, int64_t G, int64_t M, int64_t N,
                                     int64_t K, void* c, void* stream) {
-  return run_product("moe_mx4_grouped_gemm", a_codes, a_scales, a_rows, row_index, nullptr, row_divisor, w_codes, w_scales, offs,
+  return run_product("moe_mx4_grouped_gemm", a_codes, a_scales, a_rows, row_index, row_divisor, w_codes, w_scales, offs,
                      G, M, N, K, c, nullptr, nullptr, MX4_PLAIN, stream);
 }
 
@@ -273,13 +268,12 @@ extern "C" int moe_mx4_grouped_swiglu(const void* a_codes, const void* a_scales,
                                       const int32_t* row_index, int64_t row_divisor, const void* w_codes,
                                       const void* w_scales, const int32_t* offs, int64_t G, int64_t M, int64_t I,
                                       int64_t K, void* act, void* act_codes, void* act_scales, void* stream) {
-  return run_product("moe_mx4_grouped_swiglu", a_codes, a_scales, a_rows, row_index, nullptr, row_divisor, w_codes, w_scales,
+  return run_product("moe_mx4_grouped_swiglu", a_codes, a_scales, a_rows, row_index, row_divisor, w_codes, w_scales,
                      offs, G, M, I, K, act, act_codes, act_scales, act_codes ? MX4_SWIGLU_MX4 : MX4_SWIGLU, stream);
 }
 
 namespace {
-// Up to so many slots are multiplied one by one, in their own order (mx4_few.hip): without the sort and the search for
-// tiles UNSORTED_TIMES
+// Up to so many slots go one by one, in their own order (mx4_few.hip).
 constexpr int64_t kUnsortedSlots = 64;
 
 // The experts' workspace, each part 256-byte aligned.
@@ -300,18 +294,20 @@ ExpertsSpace experts_space(bool is_f32, int64_t T, int64_t H, int64_t k, int64_t
     return here;
   };
   s.f32_rows = is_f32 || S * H <= (1ll << 22);
-  s.sorted = S > kUnsortedSlots || !s.f32_rows;
-  s.perm = take(4 * S);
-  s.pos = take(4 * S);
-  s.counts = take(4 * E);
-  s.offsets = take(4 * E);
-  s.sort_bytes = moe_permute_workspace_bytes(S, E);
-  s.sort = take(static_cast<int64_t>(s.sort_bytes));
-  s.x = take(T * (H / 2));
-  s.x_scales = take(T * mx4_pitch(H));
+  s.sorted = S > kUnsortedSlots;
   s.act = take(S * (I / 2));
   s.act_scales = take(S * mx4_pitch(I));
-  s.y = take(S * H * (s.f32_rows ? 4 : 2));
+  if (s.sorted) {
+    s.perm = take(4 * S);
+    s.pos = take(4 * S);
+    s.counts = take(4 * E);
+    s.offsets = take(4 * E);
+    s.sort_bytes = moe_permute_workspace_bytes(S, E);
+    s.sort = take(static_cast<int64_t>(s.sort_bytes));
+    s.x = take(T * (H / 2));
+    s.x_scales = take(T * mx4_pitch(H));
+    s.y = take(S * H * (s.f32_rows ? 4 : 2));
+  }
   s.bytes = at;
   return s;
 }
@@ -343,19 +339,38 @@ extern "C" int moe_mx4_experts(const void* hidden, int is_f32, const int64_t* id
   int32_t* pos = reinterpret_cast<int32_t*>(ws + s.pos);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws + s.offsets);
   const int64_t S = T * k;
-  int rc = MOE_OK;
-  if (s.sorted)
-    rc = permute_fwd_run(nullptr, T, 0, ids, k, 1, E, nullptr, perm, pos, reinterpret_cast<int32_t*>(ws + s.counts),
-                         offsets, ws + s.sort, s.sort_bytes, stream);
+  if (!s.sorted) {
+    MOE_REQUIRE(gate_up_codes && gate_up_scales && down_codes && down_scales && aligned16(gate_up_codes) &&
+                    aligned8(gate_up_scales) && aligned16(down_codes) && aligned8(down_scales),
+                MOE_ERR_INVALID, "mx4 experts: bad weight pointer");
+    MOE_REQUIRE(E < (1ll << 24) && I * H < (1ll << 31), MOE_ERR_UNSUPPORTED,
+                "mx4 experts: each expert's weights must stay below 2 GiB");
+    Mx4Gemm up{};
+    up.x = hidden;
+    up.ids = ids;
+    set_divisor(up, k);
+    up.a_rows = static_cast<int>(T);
+    up.w = static_cast<const uint8_t*>(gate_up_codes);
+    up.w_scales = static_cast<const uint8_t*>(gate_up_scales);
+    up.G = static_cast<int>(E);
+    up.rows = static_cast<int>(S);
+    up.N = static_cast<int>(I);
+    up.K = static_cast<int>(H);
+    up.c_codes = reinterpret_cast<uint8_t*>(ws + s.act);
+    up.c_scales = reinterpret_cast<uint8_t*>(ws + s.act_scales);
+    return mx4_slots(up, is_f32, static_cast<const uint8_t*>(down_codes), static_cast<const uint8_t*>(down_scales),
+                     weights, T, H, k, out, as_stream(stream));
+  }
+  int rc = permute_fwd_run(nullptr, T, 0, ids, k, 1, E, nullptr, perm, pos, reinterpret_cast<int32_t*>(ws + s.counts),
+                           offsets, ws + s.sort, s.sort_bytes, stream);
   if (rc) return rc;
-  const int64_t* own = s.sorted ? nullptr : ids;
   rc = moe_mx4_quantize(hidden, is_f32, T, H, ws + s.x, ws + s.x_scales, stream);
   if (rc) return rc;
-  rc = run_product("mx4 experts, gate and up", ws + s.x, ws + s.x_scales, T, s.sorted ? perm : nullptr, own, k,
-                   gate_up_codes, gate_up_scales, s.sorted ? offsets : nullptr, E, S, I, H, nullptr, ws + s.act, ws + s.act_scales, MX4_SWIGLU_MX4, stream);
+  rc = run_product("mx4 experts, gate and up", ws + s.x, ws + s.x_scales, T, perm, k, gate_up_codes, gate_up_scales,
+                   offsets, E, S, I, H, nullptr, ws + s.act, ws + s.act_scales, MX4_SWIGLU_MX4, stream);
   if (rc) return rc;
-  rc = run_product("mx4 experts, down", ws + s.act, ws + s.act_scales, S, nullptr, own, 1, down_codes, down_scales,
-                   s.sorted ? offsets : nullptr, E, S, H, I, ws + s.y, nullptr, nullptr, s.f32_rows ? MX4_PLAIN_F32 : MX4_PLAIN, stream);
+  rc = run_product("mx4 experts, down", ws + s.act, ws + s.act_scales, S, nullptr, 1, down_codes, down_scales, offsets,
+                   E, S, H, I, ws + s.y, nullptr, nullptr, s.f32_rows ? MX4_PLAIN_F32 : MX4_PLAIN, stream);
   if (rc) return rc;
   if (!s.f32_rows) return moe_combine_fwd(ws + s.y, pos, offsets, E, weights, T, H, k, out, stream);
   const int64_t per_row = (H / 8 + kMx4Threads - 1) / kMx4Threads;
@@ -363,12 +378,12 @@ extern "C" int moe_mx4_experts(const void* hidden, int is_f32, const int64_t* id
   const dim3 grid(static_cast<unsigned>(T * per_row)), block(kMx4Threads);
   const float* y = reinterpret_cast<const float*>(ws + s.y);
   if (is_f32)
-    hipLaunchKernelGGL(mx4_combine_kernel<float>, grid, block, 0, as_stream(stream), y,
-                       s.sorted ? pos : nullptr, offsets, ids, static_cast<int>(E), weights, static_cast<int>(H), static_cast<int>(k),
+    hipLaunchKernelGGL(mx4_combine_kernel<float>, grid, block, 0, as_stream(stream), y, pos, offsets,
+                       static_cast<int>(E), weights, static_cast<int>(H), static_cast<int>(k),
                        static_cast<int>(per_row), static_cast<float*>(out));
   else
-    hipLaunchKernelGGL(mx4_combine_kernel<bf16_t>, grid, block, 0, as_stream(stream), y,
-                       s.sorted ? pos : nullptr, offsets, ids, static_cast<int>(E), weights, static_cast<int>(H), static_cast<int>(k),
+    hipLaunchKernelGGL(mx4_combine_kernel<bf16_t>, grid, block, 0, as_stream(stream), y, pos, offsets,
+                       static_cast<int>(E), weights, static_cast<int>(H), static_cast<int>(k),
                        static_cast<int>(per_row), static_cast<bf16_t*>(out));
   return launch_status("moe_mx4_experts(combine)");
 }

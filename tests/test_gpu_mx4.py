@@ -254,7 +254,7 @@ def experts_oracle(x, idx, wts, guv, dnv):
 
 @pytest.mark.parametrize("T,H,E,k,I", [(1, 64, 8, 2, 32), (1, 2048, 128, 8, 768), (7, 256, 8, 2, 128), (48, 512, 32, 4, 160),
                                        (333, 416, 8, 3, 288), (1500, 512, 4, 2, 256), (4096, 256, 16, 2, 96),
-                                       (8, 256, 16, 8, 64), (9, 256, 16, 8, 64), (300, 256, 32, 4, 288),
+                                       (8, 256, 16, 8, 64), (9, 256, 16, 8, 64), (3, 288, 32, 16, 1312), (21, 1056, 8, 3, 96), (300, 256, 32, 4, 288),
                                        (100, 512, 64, 4, 320), (3000, 512, 8, 4, 64), (2500, 1056, 64, 2, 160)])
 def test_experts(T, H, E, k, I):
     g = gen(T + H)
@@ -284,7 +284,10 @@ def test_experts_routing_corners():
         within(out, *experts_oracle(x.to(dt), idx, wts, guv, dnv))
         assert not out[20].any() and not out[3].any()
     few = slice(15, 35)  # few enough slots to go without a sort, with sentinels and repeated experts among them
-    within(mx4_experts(x[few], idx[few], wts[few], gu, dn), *experts_oracle(x[few], idx[few], wts[few], guv, dnv))
+    for dt in (torch.float32, BF):
+        out = mx4_experts(x[few].to(dt), idx[few], wts[few], gu, dn)
+        assert out.dtype == dt and not out[5].any()
+        within(out, *experts_oracle(x[few].to(dt), idx[few], wts[few], guv, dnv))
     neg = idx[few].clone()
     neg[3, 1] = -1
     out = mx4_experts(x[few], neg, wts[few], gu, dn)
