@@ -87,7 +87,11 @@ def _plain_eager(args) -> bool:
 
 
 def _wants_grad(args) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(a, Tensor) and a.requires_grad for a in args)
+    if torch.is_grad_enabled():
+        for a in args:
+            if isinstance(a, Tensor) and a.requires_grad:
+                return True
+    return False
 
 
 def _direct(name: str, *args):
@@ -148,15 +152,27 @@ def _stream(t: Tensor) -> int:
     return _lib.stream_of(t)
 
 
-def _require_one_device(*tensors: Tensor | None) -> None:
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"tensors are on different devices: {sorted(map(str, devices))}")
+def _require_one_gpu(*tensors: Tensor | None) -> None:
+    """All on one GPU; an index comparison where they are."""
+    index = None
+    for t in tensors:
+        if t is not None:
+            if index is None:
+                index = t.get_device()
+            if t.get_device() != index or index < 0:
+                break
+    else:
+        return
+    _require_gpu(*tensors)
+    raise ValueError(f"tensors are on different devices: {sorted({str(t.device) for t in tensors if t is not None})}")
+
+
+_HERE = nullcontext()
 
 
 def _device(t: Tensor):
     """Makes the tensor's GPU the current one for launches on its stream (nothing to do where it is already)."""
-    return nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _ws(nbytes: int, device) -> Tensor:
@@ -175,6 +191,10 @@ def _rows16_opt(t: Tensor | None) -> Tensor | None:
 
 def _ids64(t: Tensor) -> Tensor:
     return t.to(torch.int64).contiguous()
+
+
+def _f32(t: Tensor) -> Tensor:
+    return _rows16(t if t.dtype == torch.float32 else t.float())
 
 
 # ------------------------------------------------------------------- router
@@ -675,8 +695,7 @@ def _check_residual_norm(y, residual, weight, post_weight, gate) -> int:
         if t is not None and t.shape != (H,):
             raise ValueError(f"{name} must be ({H},), got {tuple(t.shape)}")
     kind = _gate_kind(y, gate)
-    _require_gpu(y, residual, weight, post_weight, gate)
-    _require_one_device(y, residual, weight, post_weight, gate)
+    _require_one_gpu(y, residual, weight, post_weight, gate)
     return kind
 
 
@@ -850,8 +869,7 @@ def _(x):
 def mx4_dequantize(codes: Tensor, scales: Tensor, float32: bool) -> Tensor:
     """The values [..., K] of an mx4 tensor, exactly, in bfloat16 or float32 (infinity past their range)."""
     K = _check_mx4("mx4_dequantize", codes, scales)
-    _require_gpu(codes, scales)
-    _require_one_device(codes, scales)
+    _require_one_gpu(codes, scales)
     codes, scales = _rows16(codes), _rows16(scales)
     out = torch.empty(codes.shape[:-1] + (K,), dtype=torch.float32 if float32 else BF16, device=codes.device)
     with _device(codes):
@@ -876,8 +894,7 @@ def _check_mx4_product(what, a_codes, a_scales, w_codes, w_scales, offsets) -> t
     if offsets.dtype != torch.int32 or offsets.shape != (w_codes.shape[0],):
         raise ValueError(f"{what}: offsets must be int32 [{w_codes.shape[0]}] (each group's end row), got "
                          f"{offsets.dtype} {tuple(offsets.shape)}")
-    _require_gpu(a_codes, a_scales, w_codes, w_scales, offsets)
-    _require_one_device(a_codes, a_scales, w_codes, w_scales, offsets)
+    _require_one_gpu(a_codes, a_scales, w_codes, w_scales, offsets)
     return a_codes.shape[0], w_codes.shape[0], w_codes.shape[1], K
 
 
@@ -933,8 +950,7 @@ def _check_mx4_experts(hidden, top_k_index, top_k_weights, gu_codes, gu_scales, 
         raise ValueError(f"expert weights do not match: gate_up_proj ({E}, {gu_codes.shape[1]}, {H}), down_proj "
                          f"({dn_codes.shape[0]}, {dn_codes.shape[1]}, {I}), hidden {hidden.shape[1]}")
     tensors = (hidden, top_k_index, top_k_weights, gu_codes, gu_scales, dn_codes, dn_scales)
-    _require_gpu(*tensors)
-    _require_one_device(*tensors)
+    _require_one_gpu(*tensors)
     return hidden.shape[0], H, top_k_index.shape[1], E, I
 
 
@@ -945,7 +961,7 @@ def mx4_experts(hidden: Tensor, top_k_index: Tensor, top_k_weights: Tensor, gate
     through the sort's order, the act values are quantised as they are formed, and the combine sums in fp32."""
     T, H, k, E, I = _check_mx4_experts(hidden, top_k_index, top_k_weights, gate_up_codes, gate_up_scales, down_codes,
                                        down_scales)
-    ids, w = _ids64(top_k_index), _rows16(top_k_weights.float())
+    ids, w = _rows16(top_k_index if top_k_index.dtype == torch.int64 else top_k_index.long()), _f32(top_k_weights)
     weights = tuple(map(_rows16, (gate_up_codes, gate_up_scales, down_codes, down_scales)))
     f32 = int(hidden.dtype == torch.float32)
     x = _rows16(hidden)
