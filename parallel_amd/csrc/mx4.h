@@ -144,6 +144,7 @@ __device__ __forceinline__ f32x4_t mx4_mfma(const uint4& w, const uint4& a, cons
 
 // Blocks of the few-row kernel side by side over N output columns.
 inline int64_t mx4_few_columns(int64_t N, int epi) { return mx4_glu(epi) ? (N + 31) / 32 : (N + 63) / 64; }
+inline int64_t mx4_tile_columns(int64_t N, int epi) { return mx4_glu(epi) ? (N + 127) / 128 : (N + 255) / 256; }
 
 // Products of few tiles in all (mx4_few.hip).
 int mx4_few(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name);

@@ -6,6 +6,7 @@
 // moves find; the conversion instruction scales by a power of two and rounds
 // to nearest even, saturating at 6.
 #include <type_traits>
+#include <utility>
 
 #include "mx4.h"
 
@@ -160,19 +161,30 @@ void set_divisor(Mx4Gemm& p, int64_t d) {
   p.div_shift = 31 + l;
 }
 
-// Which kernel, from the rows and groups alone (the groups' own counts are on the device).
-// The few-row kernel where it needs at most 512 blocks (16 rows by 64 weight rows each) and groups are small: it
-// is then ahead of 64-row tiles or level (mx4_few.hip has the times).  Tiles of 64, 128 or 256 rows by the mean:
-// gate and up of 128 groups, 2048 x 768, at 32, 64, 96, 128, 256 and 1024 rows each take
-//   64-row tiles 37, 47, 55, 72, 129, 433 us; 128-row 42, 44, 47, 63, 120, 360; 256-row 51, 52, 55, 58, 107, 292,
-// the down products of 64 Zipf groups with 156 rows in the mean 30 us with 128 rows and 39 with 256, a uniform
-// 160 12% less with 256: routing is skewed more often than not.
+// Which kernel, from the sizes alone (the groups' own counts are on the device).
+//
+// The few-row kernel where it needs at most two blocks (16 rows by 64 weight rows each) per CU: 2048 x 2048, one
+// group, 64, 256 and 512 rows (128, 512, 1024 blocks) 7.0, 10.5 and 18.7 us against 11.3, 11.3 and 11.6 with 64-row
+// LDS tiles; gate and up of 8 to 128 rows of 8 to 28 groups 5 to 10 against 7 to 11.
+//
+// Else the tile height whose passes over the CUs cost least, the estimate being a tile for each group at the least
+// and a tile's cost 1, 1.6 and 2.5 for 64, 128 and 256 rows (2048 x 2048, one group, 1024 rows, one pass each: 12.3,
+// 15.9, 22.8 us; 16384 rows, 8, 4 and 2 passes: 71, 56, 53; gate and up of 128 groups, 2048 x 768, at 32, 64, 96, 256
+// and 1024 rows each: 37, 47, 54, 121, 413 with 64, 40, 41, 45, 103, 317 with 128, 48, 51, 54, 98, 286 with 256).
+// Over 315 products, even and Zipf groups of 1 to 1024 rows, the choice is 2% behind the best one in the mean and 31%
+// at the worst (64 Zipf groups of 256 rows in the mean: their tiles are more than estimated).
 int mx4_product(const Mx4Gemm& p, int epi, hipStream_t stream, const char* what) {
-  const int64_t mean = (static_cast<int64_t>(p.rows) + p.G - 1) / p.G;
-  const int64_t groups = p.G < p.rows ? p.G : p.rows;
-  if (mean <= 64 && (groups + (p.rows - groups) / 16) * mx4_few_columns(p.N, epi) <= 512)
-    return mx4_few(p, epi, stream, what);
-  return mx4_tile(p, epi, mean <= 56 ? 64 : mean <= 160 ? 128 : 256, stream, what);
+  const int64_t cus = device_cus(current_device()), groups = p.G < p.rows ? p.G : p.rows;
+  if ((groups + (p.rows - groups) / 16) * mx4_few_columns(p.N, epi) <= 2 * cus) return mx4_few(p, epi, stream, what);
+  const int64_t columns = mx4_tile_columns(p.N, epi);
+  int best = 0;
+  int64_t least = 0;
+  for (const auto& [height, cost] : {std::pair{64, 10}, std::pair{128, 16}, std::pair{256, 25}}) {
+    const int64_t down = (static_cast<int64_t>(p.rows) + height - 1) / height;
+    const int64_t all = ((down > groups ? down : groups) * columns + cus - 1) / cus * cost;
+    if (best == 0 || all < least) best = height, least = all;
+  }
+  return mx4_tile(p, epi, best, stream, what);
 }
 
 int run_product(const char* what, const void* a, const void* a_scales, int64_t a_rows, const int32_t* row_index,

@@ -11,17 +11,17 @@
 // line, and their two scales, one 16-bit load; each block is one of the step's
 // two MFMAs' (products may take k in any order, so no operand is laid out anew).
 //
-// Against 64-row LDS tiles (mx4_tile.hip), of which few leave most CUs idle:
-// gate and up of 8 rows of 8 groups, 2048 x 768, 6.7 against 11.2 us (6.7 MB of
-// weights: launch and latency), of 32 rows of 28 groups 13.7 against 13.4; one
-// group's 32 rows x 2048 x 2048 6.8 against 10.5, its 256 rows 21.6 against 11.5.
-//
+// Loads in flight, not bytes, bound it: 8 rows of 8 groups' gate and up, 2048 x
+// 768 (6.7 MB of weights) take 6.9 us, of which a launch is 2 and each of the
+// waves' two steps a memory latency; 64-row LDS tiles (mx4_tile.hip), of which
+// few leave most CUs idle, take 10.6.
+
 // The experts of a few tokens (Mx4Slots) need no sort: they share none to speak
 // of, so every slot (token and choice) is a tile of its own, read by its id.
 // Gate and up quantise the token's row on the way (a wave its own 256 values a
 // step, through 144 bytes of LDS); down takes a token and 16 columns a block, a
 // wave per slot, and adds the weighted slots in fp32.  One token's experts are
-// 2 launches, SLOT_TIMES.
+// 2 launches, 6.8 + 4.8 us at 2048 x 768, 8 of 128 experts.
 #include <type_traits>
 
 #include "mx4.h"

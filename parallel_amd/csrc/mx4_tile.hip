@@ -360,8 +360,8 @@ __global__ __launch_bounds__(kTileThreads) void mx4_tile_kernel(const Mx4Gemm p,
 
 template <int BM, int STAGES>
 int launch(const Mx4Gemm& p, int epi, hipStream_t stream, const char* name) {
-  const int cols = mx4_glu(epi) ? kTileN / 2 : kTileN;
-  const int n_tiles = (p.N + cols - 1) / cols;
+  static_assert(kTileN == 256, "mx4_tile_columns");
+  const int n_tiles = static_cast<int>(mx4_tile_columns(p.N, epi));
   const int64_t most = mx4_most_tiles(p.rows, p.G, BM) * n_tiles;
   MOE_REQUIRE(most < (1ll << 30), MOE_ERR_UNSUPPORTED, "%s: too many tiles", name);
   const int64_t cus = device_cus(current_device()) / kXcds * kXcds;
