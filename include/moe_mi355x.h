@@ -484,12 +484,15 @@ int moe_mx4_grouped_swiglu(const void* a_codes, const void* a_scales,
                            void* stream);
 
 /* A layer's routed experts on mx4 weights, all launches of it: the slots
- * T x k sorted by ids (ids outside [0, E) contribute nothing), hidden [T, H]
+ * T x k sorted by ids (up to 64 of them are taken in their own order; ids
+ * outside [0, E) contribute nothing), hidden [T, H]
  * (bf16, or f32 with is_f32) quantised, gate_up [E, 2I, H] with the SwiGLU
  * output quantised, down [E, H, I], and out [T, H] (hidden's type) = the
  * weights' [T, k] (f32) sum of each token's rows in fp32.  Rows of down are
  * f32 for f32 hidden states and up to 4M values, else bf16.  H and I are
- * multiples of 32, k at most 16, E at most 1024. */
+ * multiples of 32, k at most 16, E at most 1024; the quantised rows and each
+ * expert's weights stay below 2 GiB.  The workspace is 16-byte aligned and of
+ * at least that size. */
 size_t moe_mx4_experts_workspace_bytes(int is_f32, int64_t T, int64_t H,
                                        int64_t k, int64_t E, int64_t I);
 int moe_mx4_experts(const void* hidden, int is_f32, const int64_t* ids,

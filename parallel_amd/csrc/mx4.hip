@@ -287,6 +287,7 @@ extern "C" int moe_mx4_grouped_swiglu(const void* a_codes, const void* a_scales,
 namespace {
 // Up to so many slots go one by one, in their own order (mx4_few.hip).
 constexpr int64_t kUnsortedSlots = 64;
+constexpr int kMaxExperts = 1024;  // as many as the sort takes, with or without it
 
 // The experts' workspace, each part 256-byte aligned.
 struct ExpertsSpace {
@@ -340,9 +341,16 @@ extern "C" int moe_mx4_experts(const void* hidden, int is_f32, const int64_t* id
   MOE_REQUIRE(experts_sizes(T, H, k, E, I), MOE_ERR_INVALID, "mx4 experts: bad sizes (k at most %d)", kMaxSlots);
   MOE_REQUIRE(H % 32 == 0 && I % 32 == 0, MOE_ERR_UNSUPPORTED, "mx4 experts: H=%lld and I=%lld must be multiples of 32",
               (long long)H, (long long)I);
+  MOE_REQUIRE(E <= kMaxExperts, MOE_ERR_UNSUPPORTED, "mx4 experts: more than %d experts", kMaxExperts);
+  const int64_t S = T * k;
   if (T == 0) return MOE_OK;
   MOE_REQUIRE(hidden && ids && weights && out && aligned16(hidden) && aligned16(out), MOE_ERR_INVALID,
               "mx4 experts: bad pointer");
+  MOE_REQUIRE(gate_up_codes && gate_up_scales && down_codes && down_scales && aligned16(gate_up_codes) &&
+                  aligned8(gate_up_scales) && aligned16(down_codes) && aligned8(down_scales),
+              MOE_ERR_INVALID, "mx4 experts: bad weight pointer");
+  MOE_REQUIRE(T * (H / 2) < (1ll << 31) && S * (I / 2) < (1ll << 31) && I * H < (1ll << 31), MOE_ERR_UNSUPPORTED,
+              "mx4 experts: the 4-bit rows and each expert's weights must stay below 2 GiB");
   const ExpertsSpace s = experts_space(is_f32, T, H, k, E, I);
   MOE_REQUIRE(workspace && aligned16(workspace) && workspace_bytes >= s.bytes, MOE_ERR_WORKSPACE,
               "mx4 experts: workspace %zu < %zu bytes", workspace_bytes, s.bytes);
@@ -350,13 +358,7 @@ extern "C" int moe_mx4_experts(const void* hidden, int is_f32, const int64_t* id
   int32_t* perm = reinterpret_cast<int32_t*>(ws + s.perm);
   int32_t* pos = reinterpret_cast<int32_t*>(ws + s.pos);
   int32_t* offsets = reinterpret_cast<int32_t*>(ws + s.offsets);
-  const int64_t S = T * k;
   if (!s.sorted) {
-    MOE_REQUIRE(gate_up_codes && gate_up_scales && down_codes && down_scales && aligned16(gate_up_codes) &&
-                    aligned8(gate_up_scales) && aligned16(down_codes) && aligned8(down_scales),
-                MOE_ERR_INVALID, "mx4 experts: bad weight pointer");
-    MOE_REQUIRE(E < (1ll << 24) && I * H < (1ll << 31), MOE_ERR_UNSUPPORTED,
-                "mx4 experts: each expert's weights must stay below 2 GiB");
     Mx4Gemm up{};
     up.x = hidden;
     up.ids = ids;

@@ -91,6 +91,40 @@ def test_c_entry_points_check_their_arguments():
     assert glu(scales=None) == INV and glu(codes=b + 8) == INV and glu(codes=None) == INV
 
 
+def test_experts_entry_point_checks_its_arguments():
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(256)
+    b = ctypes.addressof(buf) + (16 - ctypes.addressof(buf) % 16) % 16
+    OK, INV, UNS = _lib.MOE_OK, _lib.MOE_ERR_INVALID, _lib.MOE_ERR_UNSUPPORTED
+
+    def experts(x=b, f32=0, ids=b, w=b, T=4, H=64, k=2, E=4, I=32, guc=b, gus=b, dnc=b, dns=b, out=b, ws=b, size=1 << 40):
+        return lib.moe_mx4_experts(x, f32, ids, w, T, H, k, E, I, guc, gus, dnc, dns, out, ws, size, None)
+
+    def size(f32=0, T=4, H=64, k=2, E=4, I=32):
+        return lib.moe_mx4_experts_workspace_bytes(f32, T, H, k, E, I)
+
+    assert experts(T=0, x=None, ids=None, w=None, guc=None, gus=None, dnc=None, dns=None, out=None, ws=None, size=0) == OK
+    pointers = (dict(x=None), dict(ids=None), dict(w=None), dict(out=None), dict(x=b + 8), dict(out=b + 8),
+                dict(guc=None), dict(gus=None), dict(dnc=None), dict(dns=None), dict(guc=b + 8), dict(gus=b + 4),
+                dict(dnc=b + 8), dict(dns=b + 4))
+    for bad in (dict(T=-1), dict(H=0), dict(I=0), dict(k=0), dict(k=17), dict(E=0), dict(H=1 << 21), dict(I=1 << 21),
+                dict(T=1 << 31), dict(T=1 << 28, k=8)) + pointers + tuple(dict(T=100, **p) for p in pointers):
+        assert experts(**bad) == INV, bad
+        if not any(name in bad for name in ("x", "ids", "w", "out", "guc", "gus", "dnc", "dns")):
+            assert size(**bad) == 0, bad
+    # rows that are not whole blocks, more experts than the sort takes (also where nothing is sorted), 2 GiB
+    for bad in (dict(H=48), dict(I=40), dict(E=1025), dict(E=1025, T=1), dict(H=1 << 16, I=1 << 15, T=1),
+                dict(T=1 << 26, H=64, k=1), dict(T=1 << 24, I=1 << 9, k=8)):
+        assert experts(**bad) == UNS, bad
+    for T in (4, 100):  # without and with the sort
+        for f32 in (0, 1):
+            need = size(f32, T)
+            assert need > 0
+            assert experts(T=T, f32=f32, size=need - 1) == _lib.MOE_ERR_WORKSPACE
+            assert experts(T=T, f32=f32, ws=None) == _lib.MOE_ERR_WORKSPACE
+            assert experts(T=T, f32=f32, ws=b + 8) == _lib.MOE_ERR_WORKSPACE
+
+
 def test_oracle_follows_the_format():
     """Blocks written out by hand: scale rule, ties, saturation, sign, NaN, packing order."""
     x = torch.zeros(3, 32)
