@@ -18,33 +18,56 @@
 //
 // Both are bound by the row streams (forward 4, backward 6, or 5 where dy and
 // d_residual are the same numbers and the caller takes one tensor for both).
-// A row is held in registers, by one wave (H <= 512) or by a block of four
-// (WPR waves per row, NC 8-value chunks per lane); the backward's waves walk
-// several rows and keep the column sums in registers, so that the partials
-// are a few thousandths of the streams, and one more launch adds the partial
-// rows in a fixed order: no atomics, the same bits every time.
+// A row is held in registers, by one wave (H <= 512) or by a block of four or,
+// backward above 4096, eight (WPR waves per row, NC 8-value chunks per lane).
+// The backward's waves walk several rows, as many walkers as run at once, and
+// keep the column sums in registers, so that the partials are a few
+// thousandths of the streams, and one more launch adds the partial rows in a
+// fixed order: no atomics, the same bits every time.  The sums' registers leave
+// two or three waves per SIMD, too few to hide a row's loads behind the others'
+// sums, so the next row's loads are issued before this one's sums.
+//
+// Measured, inputs not in cache (a copy of 1 GiB: 5.1 TB/s): forward 16384 x
+// 2048 bf16 49 us (268 MB), 8192 x 8192 101 us (537 MB); backward 71 (336 MB)
+// and 132 (671 MB).  Backward with post and a gate per token: 5003 x 4096 70 us
+// (246 MB), 90 with each row's loads behind the last one's stores; 16384 x 2048
+// 103 against 121; 8192 x 8192 190 against 350 with four waves a row, whose 256
+// registers leave one wave per SIMD.  The plain sum of one chunk a lane has
+// registers for five waves and loses by it (73 against 71): it does not.
 #include <type_traits>
 
 #include "common.h"
 
 namespace moe {
 
-constexpr int kRnThreads = 256;
 enum { kGateNone = 0, kGateToken = 1, kGateChannel = 2, kGateFull = 3 };
 
+// Eight values as they are stored.
+template <class T>
+struct RnRaw {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) v[j] = reinterpret_cast<const uint4*>(p)[j];
+  }
+  __device__ __forceinline__ void values(float (&f)[8]) const {
+    if constexpr (std::is_same<T, float>::value) {
+      const float4 a = __builtin_bit_cast(float4, v[0]), b = __builtin_bit_cast(float4, v[1]);
+      f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+      f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    } else {
+      f[0] = lo_bf16(v[0].x); f[1] = hi_bf16(v[0].x);
+      f[2] = lo_bf16(v[0].y); f[3] = hi_bf16(v[0].y);
+      f[4] = lo_bf16(v[0].z); f[5] = hi_bf16(v[0].z);
+      f[6] = lo_bf16(v[0].w); f[7] = hi_bf16(v[0].w);
+    }
+  }
+};
 template <class T>
 __device__ __forceinline__ void rn_load8(const T* p, float (&f)[8]) {
-  if constexpr (std::is_same<T, float>::value) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    f[0] = lo_bf16(v.x); f[1] = hi_bf16(v.x);
-    f[2] = lo_bf16(v.y); f[3] = hi_bf16(v.y);
-    f[4] = lo_bf16(v.z); f[5] = hi_bf16(v.z);
-    f[6] = lo_bf16(v.w); f[7] = hi_bf16(v.w);
-  }
+  RnRaw<T> raw;
+  raw.load(p);
+  raw.values(f);
 }
 template <class T>
 __device__ __forceinline__ void rn_store8(T* p, const float (&f)[8]) {
@@ -67,12 +90,15 @@ __device__ __forceinline__ void rn_store1(T* p, float v) {
   else *p = f32_to_bf16(v);
 }
 
-// Sums over a row's lanes.  Four waves exchange their sums through one of two
-// LDS slots in turn: a slot is written again only after the barrier of the
+// Threads per block: a row's waves (WPR of them), four rows of one wave each.
+constexpr int rn_threads(int wpr) { return wpr > 4 ? wpr * kWave : 4 * kWave; }
+
+// Sums over a row's lanes.  A row's waves exchange their sums through one of
+// two LDS slots in turn: a slot is written again only after the barrier of the
 // sum between, which every wave reaches after it has read the slot.
 template <int WPR>
 struct RowSum {
-  float2 (*slots)[4];
+  float2 (*slots)[WPR];
   int turn;
   __device__ __forceinline__ float2 operator()(float a, float b) {
     a = wave_sum(a);
@@ -84,7 +110,10 @@ struct RowSum {
       turn ^= 1;
       if ((threadIdx.x & (kWave - 1)) == 0) s[threadIdx.x >> 6] = make_float2(a, b);
       __syncthreads();
-      return make_float2((s[0].x + s[1].x) + (s[2].x + s[3].x), (s[0].y + s[1].y) + (s[2].y + s[3].y));
+      float2 sum = s[0];
+#pragma unroll
+      for (int w = 1; w < WPR; ++w) sum = make_float2(sum.x + s[w].x, sum.y + s[w].y);
+      return sum;
     }
   }
 };
@@ -98,12 +127,12 @@ struct RnFwd {
 };
 
 template <class E, int NC, int WPR>
-__global__ __launch_bounds__(kRnThreads) void residual_norm_fwd_kernel(const RnFwd p) {
-  __shared__ float2 slots[2][4];
+__global__ __launch_bounds__(rn_threads(WPR)) void residual_norm_fwd_kernel(const RnFwd p) {
+  __shared__ float2 slots[2][WPR];
   RowSum<WPR> row_sum{slots, 0};
   constexpr int kLanes = WPR * kWave;
   const int lane = threadIdx.x % kLanes;
-  const int t = blockIdx.x * (kRnThreads / kLanes) + threadIdx.x / kLanes;  // one row per block where WPR is 4
+  const int t = blockIdx.x * (rn_threads(WPR) / kLanes) + threadIdx.x / kLanes;  // one row per block where WPR is 4
   if (t >= p.T) return;
   const int n = p.H / 8;
   const int64_t base = static_cast<int64_t>(t) * p.H;
@@ -183,13 +212,13 @@ struct RnBwd {
 
 // EXTRA: 0 the plain sum, whose registers are all it keeps; 1 with post or a gate; 2 with a gate per channel.
 template <class E, int NC, int WPR, int EXTRA>
-__global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnBwd p) {
-  __shared__ float2 slots[2][4];
+__global__ __launch_bounds__(rn_threads(WPR)) void residual_norm_bwd_kernel(const RnBwd p) {
+  __shared__ float2 slots[2][WPR];
   RowSum<WPR> row_sum{slots, 0};
   constexpr int kLanes = WPR * kWave;
   constexpr bool WHOLE = EXTRA > 0, channel = EXTRA == 2;
   const int lane = threadIdx.x % kLanes;
-  const int part = blockIdx.x * (kRnThreads / kLanes) + threadIdx.x / kLanes;
+  const int part = blockIdx.x * (rn_threads(WPR) / kLanes) + threadIdx.x / kLanes;
   if (part >= p.parts) return;
   const int n = p.H / 8;
   const float inv_h = 1.0f / static_cast<float>(p.H);
@@ -203,10 +232,31 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnB
       if constexpr (WHOLE) sum_post[i][e] = 0.0f;
       if constexpr (channel) sum_gate[i][e] = 0.0f;
     }
+  // A row as it is read.  Where registers allow, the next row's loads are in flight while this one is summed.
+  constexpr bool AHEAD = NC > 1 || EXTRA > 0;
+  RnRaw<E> y_in[NC], res_in[NC], dx_in[NC], dh_in[NC];
+  float r_in = 0.0f, ry_in = 1.0f, gt_in = 1.0f;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const int64_t base = static_cast<int64_t>(t) * p.H;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = lane + i * kLanes;
+      if (c < n) {
+        y_in[i].load(static_cast<const E*>(p.y) + base + 8 * c);
+        res_in[i].load(static_cast<const E*>(p.residual) + base + 8 * c);
+        if (p.d_x) dx_in[i].load(static_cast<const E*>(p.d_x) + base + 8 * c);
+        if (p.d_hidden) dh_in[i].load(static_cast<const E*>(p.d_hidden) + base + 8 * c);
+      }
+    }
+    r_in = p.rstd[t];
+    if (post) ry_in = p.rstd_y[t];
+    if (WHOLE && p.gate_kind == kGateToken) gt_in = rn_load1(static_cast<const E*>(p.gate) + t);
+  };
+  if (AHEAD && part < p.T) fetch(part);
   for (int t = part; t < p.T; t += p.parts) {  // the same count for every wave of a row: barriers match
     const int64_t base = static_cast<int64_t>(t) * p.H;
-    const float r = p.rstd[t], ry = post ? p.rstd_y[t] : 1.0f;
-    const float gt = WHOLE && p.gate_kind == kGateToken ? rn_load1(static_cast<const E*>(p.gate) + t) : 1.0f;
+    if (!AHEAD) fetch(t);
+    const float r = r_in, ry = ry_in, gt = gt_in;
     const E* gr = static_cast<const E*>(p.gate) + (p.gate_kind == kGateFull ? base : 0);
     float yv[NC][8], h[NC][8], dh[NC][8];
     float dot = 0.0f;
@@ -214,11 +264,11 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnB
     for (int i = 0; i < NC; ++i) {
       const int c = lane + i * kLanes;
       if (c < n) {
-        rn_load8(static_cast<const E*>(p.y) + base + 8 * c, yv[i]);
-        rn_load8(static_cast<const E*>(p.residual) + base + 8 * c, h[i]);
+        y_in[i].values(yv[i]);
+        res_in[i].values(h[i]);
         float w[8], g[8], v[8], dx[8];
-        if (p.d_x) rn_load8(static_cast<const E*>(p.d_x) + base + 8 * c, dx);
-        if (p.d_hidden) rn_load8(static_cast<const E*>(p.d_hidden) + base + 8 * c, dh[i]);
+        if (p.d_x) dx_in[i].values(dx);
+        if (p.d_hidden) dh_in[i].values(dh[i]);
         else
 #pragma unroll
           for (int e = 0; e < 8; ++e) dh[i][e] = 0.0f;
@@ -252,6 +302,7 @@ __global__ __launch_bounds__(kRnThreads) void residual_norm_bwd_kernel(const RnB
         }
       }
     }
+    if (AHEAD && t + p.parts < p.T) fetch(t + p.parts);
     if (p.d_x) {
       const float k = r * r * r * inv_h * row_sum(dot, 0.0f).x;
 #pragma unroll
@@ -394,13 +445,13 @@ int64_t rn_parts(int64_t T, int64_t H, int64_t blocks) {
   return T < 1 ? 1 : T < most ? T : most;
 }
 
-template <class F>
+template <bool BWD, class F>
 void rn_dispatch(int64_t H, F&& f) {
   using std::integral_constant;
   if (wave_rows(H)) f(integral_constant<int, 1>{}, integral_constant<int, 1>{});
   else if (H <= 2048) f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
   else if (H <= 4096) f(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-  else f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+  else f(integral_constant<int, BWD ? 2 : 4>{}, integral_constant<int, BWD ? 8 : 4>{});
 }
 }  // namespace
 
@@ -416,13 +467,13 @@ extern "C" int moe_residual_norm_fwd(const void* y, const void* residual, const 
               "residual_norm fwd: bad output pointer");
   const RnFwd p{y,      residual, post, gate, gamma, gate_kind, static_cast<int>(T), static_cast<int>(H), branch_scale,
                 residual_scale, eps, hidden, x, rstd_y, rstd};
-  rn_dispatch(H, [&](auto nc, auto wpr) {
-    constexpr int NC = decltype(nc)::value, WPR = decltype(wpr)::value, per = 4 / WPR;
+  rn_dispatch<false>(H, [&](auto nc, auto wpr) {
+    constexpr int NC = decltype(nc)::value, WPR = decltype(wpr)::value, per = rn_threads(WPR) / (WPR * kWave);
     const dim3 grid(static_cast<unsigned>((T + per - 1) / per));
     if (is_f32)
-      hipLaunchKernelGGL((residual_norm_fwd_kernel<float, NC, WPR>), grid, dim3(kRnThreads), 0, as_stream(stream), p);
+      hipLaunchKernelGGL((residual_norm_fwd_kernel<float, NC, WPR>), grid, dim3(rn_threads(WPR)), 0, as_stream(stream), p);
     else
-      hipLaunchKernelGGL((residual_norm_fwd_kernel<bf16_t, NC, WPR>), grid, dim3(kRnThreads), 0, as_stream(stream), p);
+      hipLaunchKernelGGL((residual_norm_fwd_kernel<bf16_t, NC, WPR>), grid, dim3(rn_threads(WPR)), 0, as_stream(stream), p);
   });
   return launch_status("moe_residual_norm_fwd");
 }
@@ -458,15 +509,15 @@ extern "C" int moe_residual_norm_bwd(const void* d_hidden, const void* d_x, cons
   RnBwd p{d_hidden, d_x, y, residual, post, gate, gamma, rstd_y, rstd, gate_kind, static_cast<int>(T),
           static_cast<int>(H), 0, branch_scale, residual_scale, d_y, d_residual, d_gate,
           static_cast<float*>(workspace)};
-  rn_dispatch(H, [&](auto nc, auto wpr) {  // (with T == 0 the one walker writes its zero sums)
-    constexpr int NC = decltype(nc)::value, WPR = decltype(wpr)::value, per = 4 / WPR;
+  rn_dispatch<true>(H, [&](auto nc, auto wpr) {  // (with T == 0 the one walker writes its zero sums)
+    constexpr int NC = decltype(nc)::value, WPR = decltype(wpr)::value, per = rn_threads(WPR) / (WPR * kWave);
     auto launch = [&](auto e, auto extra) {
       const auto kernel = residual_norm_bwd_kernel<decltype(e), NC, WPR, decltype(extra)::value>;
       const int dev = current_device();
       const int64_t fit = static_cast<int64_t>(device_cus(dev)) *
-                          cached_blocks_per_cu(dev, reinterpret_cast<const void*>(kernel), kRnThreads, 0);
+                          cached_blocks_per_cu(dev, reinterpret_cast<const void*>(kernel), rn_threads(WPR), 0);
       p.parts = static_cast<int>(rn_parts(T, H, fit < kRnBlocks ? fit : kRnBlocks));
-      hipLaunchKernelGGL(kernel, dim3((p.parts + per - 1) / per), dim3(kRnThreads), 0, as_stream(stream), p);
+      hipLaunchKernelGGL(kernel, dim3((p.parts + per - 1) / per), dim3(rn_threads(WPR)), 0, as_stream(stream), p);
     };
     auto typed = [&](auto e) {
       if (channel) launch(e, std::integral_constant<int, 2>{});

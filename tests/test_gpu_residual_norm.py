@@ -148,6 +148,13 @@ def test_more_rows_than_walkers(T, H, gate, post, dtype):
     compare(t, d_hidden, d_x, 1.0, 1.0)
 
 
+@pytest.mark.parametrize("T,H,gate", [(700, 4096, "token"), (600, 5008, "channel"), (600, 8192, "full"), (1, 8192, "token")])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_several_wide_rows_per_walker_with_post(T, H, gate, dtype):
+    t, d_hidden, d_x = make(T, H, dtype, True, gate)
+    compare(t, d_hidden, d_x, 0.7, 1.2)
+
+
 @pytest.mark.parametrize("gate,post,bs", [("none", False, 1.0), ("none", False, 0.5), ("token", True, 0.5)])
 @pytest.mark.parametrize("which", ["hidden", "x"])
 def test_one_output_alone_has_a_gradient(which, gate, post, bs):
