@@ -208,7 +208,7 @@ int moe_rmsnorm_bwd(const void* dx, const void* dx2, const void* h,
  * column (gate[H]), 3 one per element (gate[T,H]).  All operands bf16, or all
  * f32 with is_f32; rstd_y[T] (written with post only) and rstd[T] are f32,
  * either may be NULL (the backward needs them).
- * H a multiple of 8, at most 8192.  For eps = 1e-6, equal scales of 1, no post
+ * H a multiple of 8, at most 8192; T at most 2^30.  For eps = 1e-6, equal scales of 1, no post
  * and no gate, hidden and x are the sum and the norm of
  * TF/models/qwen3_moe/modeling_qwen3_moe.py:340-345 with one rounding. */
 int moe_residual_norm_fwd(const void* y, const void* residual, const void* post,

@@ -420,7 +420,8 @@ constexpr int64_t kRnMaxH = 8192;
 
 int check_rn(const char* what, const void* y, const void* residual, const void* gate, int gate_kind, const void* gamma,
              const void* post, int64_t T, int64_t H) {
-  MOE_REQUIRE(T >= 0 && T < (1ll << 31), MOE_ERR_INVALID, "%s: bad row count %lld", what, (long long)T);
+  // (a walker's next row, at most 4096 on, stays an int)
+  MOE_REQUIRE(T >= 0 && T <= (1ll << 30), MOE_ERR_INVALID, "%s: bad row count %lld", what, (long long)T);
   MOE_REQUIRE(H > 0 && H % 8 == 0 && H <= kRnMaxH, MOE_ERR_UNSUPPORTED,
               "%s: H=%lld must be a multiple of 8 and at most %lld", what, (long long)H, (long long)kRnMaxH);
   MOE_REQUIRE(gate_kind >= kGateNone && gate_kind <= kGateFull, MOE_ERR_INVALID, "%s: bad gate kind %d", what,

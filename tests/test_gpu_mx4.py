@@ -182,6 +182,21 @@ def test_larger_products(rows, G, N, K):
     within(mx4_swiglu(a, w, offsets_of(counts)), *O.swiglu(want, err), "swiglu")
 
 
+# Sizes whose passes over 256 CUs take 128-row tiles (16 tiles down by 16 across), 256-row tiles (16 by 16 of those), and
+# the few-row kernel for many rows of a narrow product; whole and broken stages of K, groups with a row or none.
+@pytest.mark.parametrize("rows,N", [(2000, 2000), (1990, 1928), (4000, 2000), (4090, 1928), (4096, 40), (1500, 96)])
+@pytest.mark.parametrize("K,counts", [(32, [1.0]), (544, [0.3, 0.0, 0.001, 0.6]), (768, [1 / 9] * 9), (288, [0.0, 0.97, 0.0, 0.001])])
+def test_passes_over_the_card(rows, N, K, counts):
+    counts = [int(c * rows) for c in counts]
+    rows = sum(counts)
+    g = gen(rows + K)
+    a, av = operand(g, rows, K)
+    w, wv = operand(g, len(counts), 2 * N, K, std=0.1)
+    want, err = O.product(av, wv, counts)
+    within(mx4_grouped_mm(a, w, offsets_of(counts)), want, err, "mm")
+    within(mx4_swiglu(a, w, offsets_of(counts)), *O.swiglu(want, err), "swiglu")
+
+
 def test_nan_blocks_reach_their_rows_and_columns_alone():
     g = gen(8)
     counts = [20, 0, 50]
@@ -261,6 +276,19 @@ def test_experts(T, H, E, k, I):
     gu, guv, dn, dnv = layer(g, E, H, I)
     x = (torch.randn(T, H, generator=g, device=DEV) * 2).to(BF)
     top = torch.topk(torch.randn(T, E, generator=g, device=DEV), k, dim=1)
+    wts = torch.softmax(top.values, 1)
+    within(mx4_experts(x, top.indices, wts, gu, dn), *experts_oracle(x, top.indices, wts, guv, dnv))
+
+
+# The same with the act values quantised and the rows of down in bf16 (bf16 hidden states of this size) and fp32.
+@pytest.mark.parametrize("T", [500, 1013])
+@pytest.mark.parametrize("dtype", [BF, torch.float32], ids=["bf16", "fp32"])
+def test_experts_on_tall_tiles(T, dtype):
+    E, H, k, I = 6, 4000, 4, 1984
+    g = gen(T)
+    gu, guv, dn, dnv = layer(g, E, H, I)
+    x = (torch.randn(T, H, generator=g, device=DEV) * 2).to(dtype)
+    top = torch.topk(torch.randn(T, E, generator=g, device=DEV) - torch.arange(E, device=DEV) * 0.5, k, dim=1)
     wts = torch.softmax(top.values, 1)
     within(mx4_experts(x, top.indices, wts, gu, dn), *experts_oracle(x, top.indices, wts, guv, dnv))
 
