@@ -171,6 +171,8 @@ void set_divisor(Mx4Gemm& p, int64_t d) {
 // and a tile's cost 1, 1.6 and 2.5 for 64, 128 and 256 rows (2048 x 2048, one group, 1024 rows, one pass each: 12.3,
 // 15.9, 22.8 us; 16384 rows, 8, 4 and 2 passes: 71, 56, 53; gate and up of 128 groups, 2048 x 768, at 32, 64, 96, 256
 // and 1024 rows each: 37, 47, 54, 121, 413 with 64, 40, 41, 45, 103, 317 with 128, 48, 51, 54, 98, 286 with 256).
+// Up to K 1024, where the epilogue is more of a tile, a 128-row tile costs two of 64 rows and is not taken (down, K 768,
+// 64 even groups of 128 and 256 rows 24 and 37 us with 64, 26 and 37 with 128; Zipf ones 25 and 40, 27 and 38).
 // Over 315 products, even and Zipf groups of 1 to 1024 rows, the choice is 2% behind the best one in the mean and 31%
 // at the worst (64 Zipf groups of 256 rows in the mean: their tiles are more than estimated).
 int mx4_product(const Mx4Gemm& p, int epi, hipStream_t stream, const char* what) {
@@ -179,7 +181,7 @@ int mx4_product(const Mx4Gemm& p, int epi, hipStream_t stream, const char* what)
   const int64_t columns = mx4_tile_columns(p.N, epi);
   int best = 0;
   int64_t least = 0;
-  for (const auto& [height, cost] : {std::pair{64, 10}, std::pair{128, 16}, std::pair{256, 25}}) {
+  for (const auto& [height, cost] : {std::pair{64, 10}, std::pair{128, p.K > 1024 ? 16 : 20}, std::pair{256, 25}}) {
     const int64_t down = (static_cast<int64_t>(p.rows) + height - 1) / height;
     const int64_t all = ((down > groups ? down : groups) * columns + cus - 1) / cus * cost;
     if (best == 0 || all < least) best = height, least = all;

@@ -182,10 +182,10 @@ def test_larger_products(rows, G, N, K):
     within(mx4_swiglu(a, w, offsets_of(counts)), *O.swiglu(want, err), "swiglu")
 
 
-# Sizes whose passes over 256 CUs take 128-row tiles (16 tiles down by 16 across), 256-row tiles (16 by 16 of those), and
-# the few-row kernel for many rows of a narrow product; whole and broken stages of K, groups with a row or none.
+# Sizes whose passes over 256 CUs take 128-row tiles (K over 1024; 16 tiles down by 16 across), 256-row tiles (16 by 16
+# of those), and the few-row kernel for many rows of a narrow product; whole and broken stages of K, groups with a row or none.
 @pytest.mark.parametrize("rows,N", [(2000, 2000), (1990, 1928), (4000, 2000), (4090, 1928), (4096, 40), (1500, 96)])
-@pytest.mark.parametrize("K,counts", [(32, [1.0]), (544, [0.3, 0.0, 0.001, 0.6]), (768, [1 / 9] * 9), (288, [0.0, 0.97, 0.0, 0.001])])
+@pytest.mark.parametrize("K,counts", [(1056, [0.5, 0.0, 0.3, 0.2]), (2048, [1.0]), (32, [1.0]), (544, [0.3, 0.0, 0.001, 0.6]), (768, [1 / 9] * 9), (288, [0.0, 0.97, 0.0, 0.001])])
 def test_passes_over_the_card(rows, N, K, counts):
     counts = [int(c * rows) for c in counts]
     rows = sum(counts)
