@@ -369,6 +369,84 @@ def test_replays_of_a_captured_layer_and_another_stream():
         assert torch.equal(out, mx4_experts(x, idx, wts, gu, dn)), n
 
 
+def test_two_streams_and_two_graphs_at_once():
+    g = gen(22)
+    E, H, I = 32, 512, 256
+    gu, _, dn, _ = layer(g, E, H, I)
+    cases = []
+    for T in (5, 7, 600):  # two without the sort, one with
+        top = torch.topk(torch.randn(T, E, generator=g, device=DEV), 4, dim=1)
+        cases.append((torch.randn(T, H, generator=g, device=DEV).to(BF), top.indices, torch.softmax(top.values, 1)))
+    want = [mx4_experts(*c, gu, dn) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(mx4_experts(*c, gu, dn))
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, got, want))
+    graphs, outs = [], []
+    for c in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(mx4_experts(*c, gu, dn))
+    for _ in range(3):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, outs, want))
+
+
+def test_values_past_32_bits():
+    """Quantisation of more than 2^31 values, weights of more than 2^31 bytes of codes, products and experts with more
+    than 2^31 outputs: the last part as a call on it alone gives it."""
+    g = gen(23)
+    block, other = (torch.randn(1024, 4096, generator=g, device=DEV).to(BF) for _ in range(2))
+    x = block.repeat(520, 1)
+    x[-1024:] = other
+    assert x.numel() > 1 << 31
+    q, part = quantize_mx4(x), quantize_mx4(other)
+    assert torch.equal(q.codes[-1024:], part.codes) and torch.equal(q.scales[-1024:], part.scales)
+    assert torch.equal(q.dequantize()[-1024:], part.dequantize())
+    del x
+
+    w = MX4Tensor(q.codes.view(260, 2048, 2048).repeat(2, 1, 1), q.scales.view(260, 2048, 128).repeat(2, 1, 1))
+    assert w.codes.numel() > 1 << 31
+    tail, tailv = operand(g, 8, 2048, 4096, std=0.1)
+    w.codes[-8:], w.scales[-8:] = tail.codes, tail.scales
+    a, av = operand(g, 520, 4096)
+    each = torch.arange(1, 521, dtype=torch.int32, device=DEV)  # a row a group
+    want, err = O.product(av[-8:], tailv, [1] * 8)
+    within(mx4_grouped_mm(a, w, each)[-8:], want, err, "mm")
+    within(mx4_swiglu(a, w, each)[-8:], *O.swiglu(want, err), "swiglu")
+    del w, q
+
+    rows = 1_100_000
+    a = MX4Tensor(part.codes[:, :64].repeat(rows // 1000, 1)[:rows], part.scales[:, :8].repeat(rows // 1000, 1)[:rows])
+    w, _ = operand(g, 2, 2048, 128)
+    offs = offsets_of([rows - 5000, 5000])
+    out = mx4_grouped_mm(a, w, offs)
+    assert out.numel() > 1 << 31
+    last = MX4Tensor(a.codes[-5000:].contiguous(), a.scales[-5000:].contiguous())
+    assert torch.equal(out[-5000:], mx4_grouped_mm(last, w, offsets_of([0, 5000])))
+    del out, a
+
+    T, E, H, I, k = 140_000, 16, 2048, 64, 8
+    assert T * k * H > 1 << 31
+    gu, _, dn, _ = layer(g, E, H, I)
+    x = block[:, :H].repeat(140, 1)[:T].contiguous()
+    idx = torch.topk(torch.randn(T, E, generator=g, device=DEV), k, dim=1).indices
+    wts = torch.rand(T, k, generator=g, device=DEV)
+    out = mx4_experts(x, idx, wts, gu, dn)
+    tail = 4000  # (rows of down in bf16 for it too)
+    assert torch.equal(out[-tail:], mx4_experts(x[-tail:], idx[-tail:], wts[-tail:], gu, dn))
+    del out, x
+    torch.cuda.empty_cache()
+
+
 def test_modules_run_together_between_two_blocks():
     """Residual norm, router, experts on 4-bit weights, residual norm: the layer's second half as inference runs it."""
     g = gen(30)

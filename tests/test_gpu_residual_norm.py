@@ -2,7 +2,8 @@
 
 The oracle is the formula in float64.  Tolerances are counted, not fitted: u = 2^-24 is half a step of fp32, and
 every value that the kernel forms carries the bound of its error along (class V).  A row sum adds at most 32 values
-in a lane, 6 levels of lanes and 2 of waves, so it is off by at most 40 u of the sum of sizes; a column sum adds
+in a lane (31 sums), 6 levels of lanes and 3 more waves (16 values and 7 where eight waves share a row), so it is off
+by at most 40 u of the sum of sizes; a column sum adds
 ceil(T / walkers) rows in a walker, 64 to 256 walkers in a thread and 16 threads.  A product or sum of computed
 values rounds once more; rsqrt is within 2 u and counts 4 with its argument.  The output rounds by 2^-8 (bf16) or
 2^-24 (fp32) of the value.
@@ -271,3 +272,78 @@ def test_the_op_under_tracing_gives_the_same():
     plain = run({k: v.detach() for k, v in t.items()}, d_hidden, d_x, 0.3, 1.0)
     for name, value in zip(("y", "residual", "weight", "post_weight", "gate"), grads):
         assert torch.equal(value, plain[name]), name
+
+
+def test_one_tensor_in_several_places():
+    """y and residual the same leaf, the gate too, and one weight for both norms: the places' gradients add up."""
+    t, d_hidden, d_x = make(37, 640, torch.float32, True, "full")
+    t["residual"], t["gate"], t["post_weight"] = t["y"], t["y"], t["weight"]
+    parts = run(t, d_hidden, d_x, 0.4, 1.1)
+    y, w = t["y"].clone().requires_grad_(), t["weight"].clone().requires_grad_()
+    hidden, x = residual_norm(y, y, w, post_weight=w, gate=y, branch_scale=0.4, residual_scale=1.1)
+    torch.autograd.backward([hidden, x], [d_hidden, d_x])
+    assert torch.equal(hidden, parts["hidden"]) and torch.equal(x, parts["x"])
+    for got, names in ((y.grad, ("y", "residual", "gate")), (w.grad, ("weight", "post_weight"))):
+        each = [parts[n].double() for n in names]
+        bound = 2 * U * sum(e.abs() for e in each) * (1 + U)  # two fp32 sums, in any order
+        assert ((got.double() - sum(each)).abs() <= bound).all()
+
+
+def test_gradients_accumulate_apart_where_one_tensor_serves_two():
+    """The plain sum's one gradient of y and residual: a second pass into .grad, and one changed in place."""
+    t, d_hidden, d_x = make(24, 256, torch.float32, False, "none")
+    once = run(t, d_hidden, d_x, 1.0, 1.0)
+    leaves = [t[n].clone().requires_grad_() for n in ("y", "residual", "weight")]
+    for _ in range(2):
+        torch.autograd.backward(residual_norm(*leaves), [d_hidden, d_x])
+    for leaf, name in zip(leaves, ("y", "residual", "weight")):
+        assert torch.equal(leaf.grad, 2 * once[name]), name
+    leaves[0].grad.zero_()
+    assert torch.equal(leaves[1].grad, 2 * once["residual"])
+
+
+def test_two_streams_and_two_graphs_at_once():
+    cases = [make(700, 1024, torch.bfloat16, True, "channel", seed=s) for s in (1, 2)]
+    want = [run(*c, 0.3, 1.0) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(run(*c, 0.3, 1.0))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            for name in w:
+                assert torch.equal(g[name], w[name]), name
+    graphs, outs = [], []
+    for c in cases:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(*c, 0.3, 1.0))
+    for _ in range(3):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(outs, want):
+            for name in w:
+                assert torch.equal(g[name], w[name]), name
+
+
+def test_rows_past_32_bits():
+    """More than 2^31 values a tensor: the last rows as a call on them alone gives them."""
+    T, H, tail = 270_000, 8192, 300
+    assert T * H > 1 << 31
+    block = torch.randn(1000, H, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV).to(torch.bfloat16)
+    big = lambda k: block.roll(k, 0).repeat(T // 1000, 1)  # noqa: E731
+    y, residual, d_hidden, d_x = (big(k) for k in range(4))
+    w, p = (1 + 0.1 * block[k] for k in range(2))
+    t = dict(y=y, residual=residual, weight=w, post_weight=p, gate=block[:, :1].repeat(T // 1000, 1))
+    got = run(t, d_hidden, d_x, 0.5, 1.0)
+    last = {k: v if k in ("weight", "post_weight") else v[-tail:] for k, v in t.items()}
+    want = run(last, d_hidden[-tail:], d_x[-tail:], 0.5, 1.0)
+    for name in ("hidden", "x", "y", "residual", "gate"):
+        assert torch.equal(got[name][-tail:], want[name]), name
+    del got, want, y, residual, d_hidden, d_x, t, last
+    torch.cuda.empty_cache()
