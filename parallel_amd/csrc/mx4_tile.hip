@@ -9,9 +9,9 @@
 // 16) and + 1 of a stage's row, so its two codes chunks are neighbours and its
 // two scales one 16-bit read.  The scales come 16 bytes (two stages) of a row
 // at a time into a ring of their own: fetched stage by stage they were as many
-// L2 requests as the codes' whole lines.  The wave's 64 weight rows are dealt to its four
-// fragments four rows at a time, so that a lane's results are twice 8 (with
-// swiglu once) neighbouring output columns of one row, stored as they are.
+// L2 requests as the codes' whole lines.  The wave's 64 weight rows are dealt to
+// its four fragments four rows at a time, so that a lane's results are twice 8
+// (with swiglu once) neighbouring output columns of one row, stored as they are.
 //
 // Blocks are persistent, one per CU, and run one stream of stages over their
 // tiles: a DMA cursor (buffer_load ... lds, fired between the products) fills a
@@ -20,6 +20,14 @@
 // output is written.  The epilogue issues the same number of stores whatever is
 // in range (out of range ones are dropped by the buffer resource), so that the
 // waits that follow can leave them in flight.
+//
+// Measured at 1024 rows of each of 128 groups: gate and up, 2048 x 768, 308 us
+// (825 GFLOP, 2.7 PFLOP/s), down with bf16 rows 235 (537 MB written).  Parts
+// switched off: LDS reads alone 79 us of gate and up's, with the products 193
+// (bare products 142 at the power limit), with the DMA 250; the rest is the
+// epilogue, which nothing covers: one tile's results fill the registers, and
+// two blocks of half the rows per CU lost as much to the L1's bytes (344).
+// Where weights stream once (384 rows) it is HBM: 41 us for 204 MB.
 #include "dma.h"
 #include "mx4.h"
 
