@@ -484,8 +484,8 @@ int moe_mx4_grouped_swiglu(const void* a_codes, const void* a_scales,
                            void* stream);
 
 /* A layer's routed experts on mx4 weights, all launches of it: the slots
- * T x k sorted by ids (up to 64 of them are taken in their own order; ids
- * outside [0, E) contribute nothing), hidden [T, H]
+ * T x k sorted by ids (up to 128 that hardly share experts are taken in their
+ * own order; ids outside [0, E) contribute nothing), hidden [T, H]
  * (bf16, or f32 with is_f32) quantised, gate_up [E, 2I, H] with the SwiGLU
  * output quantised, down [E, H, I], and out [T, H] (hidden's type) = the
  * weights' [T, k] (f32) sum of each token's rows in fp32.  Rows of down are

@@ -5,6 +5,7 @@
 // of bf16), four neighbouring lanes a block of 32, whose largest size two DPP
 // moves find; the conversion instruction scales by a power of two and rounds
 // to nearest even, saturating at 6.
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -307,8 +308,16 @@ extern "C" int moe_mx4_grouped_swiglu(const void* a_codes, const void* a_scales,
 }
 
 namespace {
-// Up to so many slots go one by one, in their own order (mx4_few.hip).
-constexpr int64_t kUnsortedSlots = 64;
+// Whether the slots go one by one, in their own order (mx4_few.hip): up to 128 that read at most 48 MB of weights again
+// which an expert's rows taken together would read once (the tokens' experts by even routing).  128 experts of 2048 x
+// 768, 8 a token: 8, 64, 96 and 128 slots (0, 33, 70, 116 MB) 12, 42, 58, 72 us against 23, 53, 60, 62 sorted; 8 of 1024
+// x 512, 2 a token: 32, 48, 64 slots (20, 33, 47 MB) 13, 17, 20 against 18 each; 16 of 4096 x 1536, 2 a token: 8, 16, 32
+// slots (15, 57, 165 MB) 26, 44, 73 against 33, 42, 47.
+bool slots_apart(int64_t T, int64_t H, int64_t k, int64_t E, int64_t I) {
+  const double slots = static_cast<double>(T) * k, share = k < E ? static_cast<double>(k) / E : 1.0;
+  const double hit = E * (1.0 - std::pow(1.0 - share, static_cast<double>(T)));
+  return slots <= 128 && (slots - hit) * (3.0 * I * H * 17 / 32) <= 48e6;
+}
 constexpr int kMaxExperts = 1024;  // as many as the sort takes, with or without it
 
 // The experts' workspace, each part 256-byte aligned.
@@ -329,7 +338,7 @@ ExpertsSpace experts_space(bool is_f32, int64_t T, int64_t H, int64_t k, int64_t
     return here;
   };
   s.f32_rows = is_f32 || S * H <= (1ll << 22);
-  s.sorted = S > kUnsortedSlots;
+  s.sorted = !slots_apart(T, H, k, E, I);
   s.act = take(S * (I / 2));
   s.act_scales = take(S * mx4_pitch(I));
   if (s.sorted) {

@@ -280,6 +280,29 @@ def test_experts(T, H, E, k, I):
     within(mx4_experts(x, top.indices, wts, gu, dn), *experts_oracle(x, top.indices, wts, guv, dnv))
 
 
+# Slots in their own order or sorted: 128 and 130 of them, many that share few experts of small and of large weights,
+# more choices than experts.
+@pytest.mark.parametrize("T,H,E,k,I", [(16, 256, 64, 8, 96), (13, 256, 64, 10, 96), (64, 512, 4, 2, 256), (16, 2048, 4, 2, 2048),
+                                       (2, 2048, 4, 2, 2048), (1, 4096, 4, 4, 2048), (128, 64, 1, 1, 32)])
+@pytest.mark.parametrize("dtype", [BF, torch.float32], ids=["bf16", "fp32"])
+def test_experts_of_few_slots(T, H, E, k, I, dtype):
+    g = gen(T + H + E)
+    gu, guv, dn, dnv = layer(g, E, H, I)
+    x = (torch.randn(T, H, generator=g, device=DEV) * 2).to(dtype)
+    top = torch.topk(torch.randn(T, E, generator=g, device=DEV), k, dim=1)
+    wts = torch.softmax(top.values, 1)
+    within(mx4_experts(x, top.indices, wts, gu, dn), *experts_oracle(x, top.indices, wts, guv, dnv))
+
+
+def test_experts_with_more_choices_than_experts():
+    g = gen(9)
+    gu, guv, dn, dnv = layer(g, 2, 128, 64)
+    x = torch.randn(5, 128, generator=g, device=DEV).to(BF)
+    idx = torch.randint(2, (5, 6), generator=g, device=DEV)
+    wts = torch.rand(5, 6, generator=g, device=DEV)
+    within(mx4_experts(x, idx, wts, gu, dn), *experts_oracle(x, idx, wts, guv, dnv))
+
+
 # The same with the act values quantised and the rows of down in bf16 (bf16 hidden states of this size) and fp32.
 @pytest.mark.parametrize("T", [500, 1013])
 @pytest.mark.parametrize("dtype", [BF, torch.float32], ids=["bf16", "fp32"])
