@@ -392,6 +392,20 @@ def test_replays_of_a_captured_layer_and_another_stream():
         assert torch.equal(out, mx4_experts(x, idx, wts, gu, dn)), n
 
 
+@pytest.mark.parametrize("rows,K", [(4097, 8192), (33000, 1056)])
+@pytest.mark.parametrize("dtype", [BF, torch.float32], ids=["bf16", "fp32"])
+def test_large_tensors_to_codes_and_back(rows, K, dtype):
+    """More than 2^25 values, the last threads' chunks in part past the end: each row as it is in a small tensor."""
+    x = torch.randn(rows, K, generator=gen(rows), device=DEV).to(dtype)
+    assert x.numel() > 1 << 25
+    q = quantize_mx4(x)
+    back = q.dequantize(dtype)
+    for lo in (0, rows // 2, rows - 70):
+        part = assert_quantized(x[lo:lo + 70])
+        assert torch.equal(q.codes[lo:lo + 70], part.codes) and torch.equal(q.scales[lo:lo + 70], part.scales)
+        assert torch.equal(back[lo:lo + 70], part.dequantize(dtype))
+
+
 def test_two_streams_and_two_graphs_at_once():
     g = gen(22)
     E, H, I = 32, 512, 256
